@@ -32,6 +32,7 @@ extern "C" {
 #define MCS_DTYPE_BF16 0
 #define MCS_DTYPE_FP16 1
 #define MCS_DTYPE_E4M3 2
+#define MCS_DTYPE_FP32 3 /* mcs_rotary only */
 
 /* Argument errors (returned, never stored in the status word). */
 #define MCS_ERR_NULL_POINTER (-1)
@@ -201,6 +202,40 @@ typedef struct mcs_qkv_epilogue_args {
 } mcs_qkv_epilogue_args;
 
 int mcs_qkv_norm_rope_scatter(const mcs_qkv_epilogue_args* args, void* stream);
+
+/*
+ * Rotary positions of one or two (B, L, H, D) tensors in one launch (q and k of a layer): rotation pair p of every row turns by
+ * w = position[axis[p]] * f_p, times a magnitude m,
+ *   y_a = m (x_a cos w - x_b sin w),  y_b = m (x_a sin w + x_b cos w),
+ * with (a, b) = (2p, 2p + 1) (layout 0, interleaved) or (p, p + n_pairs) (layout 1, half); elements from 2 * n_pairs on are
+ * copied.  `inverse` turns the other way with the same magnitude: the gradient of the rotation.  Frequencies come as
+ * turns[p] = round(2^64 * f_p / (2 pi)) modulo 2^64, so angles are exact for every int32 / int64 position, negative ones
+ * included.  turns and axis are HOST arrays of n_pairs (<= 128) entries and are copied into the launch's arguments.
+ * y may be x (same strides): in place.  H[1] = 0: one tensor.  A size of zero launches nothing.
+ *
+ * Stands beside mcs_qkv_norm_rope_scatter, which rotates inside the exchange of a context-parallel layer; the reference leaves
+ * the rotary embedding to the host model (mcsparse/h3/context_parallel.py:165-176 gets rotated q and k).
+ */
+typedef struct mcs_rotary_args {
+  const void* x[2];
+  void* y[2];
+  int64_t x_stride[2][3];     /* batch, row, head (elements); the head dimension is contiguous */
+  int64_t y_stride[2][3];
+  const void* positions;      /* int32 or int64, element (b, row, axis) at the strides below */
+  int64_t p_stride[3];
+  const uint64_t* turns;      /* host array */
+  const uint8_t* axis;        /* host array, entries < n_axes */
+  int32_t H[2];
+  int32_t B, L, D;
+  int32_t n_pairs, n_axes;    /* n_axes 1..3 */
+  int32_t layout;             /* 0 interleaved, 1 half */
+  int32_t pos64;              /* 0: positions are int32, 1: int64 */
+  int32_t inverse;
+  int32_t dtype;              /* MCS_DTYPE_BF16, MCS_DTYPE_FP16 or MCS_DTYPE_FP32 */
+  float magnitude;            /* finite */
+} mcs_rotary_args;
+
+int mcs_rotary(const mcs_rotary_args* args, void* stream);
 
 /*
  * Anchor-step group mass: mass[b,h,m,j] = sum_{i in group m} exp(scale * q_i . k_j - lse_i), fp32.

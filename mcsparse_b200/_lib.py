@@ -17,6 +17,7 @@ LIB_PATH = Path(os.environ.get("MCSPARSE_B200_LIB") or Path(__file__).resolve().
 MCS_DTYPE_BF16 = 0
 MCS_DTYPE_FP16 = 1
 MCS_DTYPE_E4M3 = 2
+MCS_DTYPE_FP32 = 3
 MCS_ATTN_OUT_GROUP_ORDER = 1
 # argument-error codes of include/mcsparse_b200.h
 MCS_ERR_NULL_POINTER, MCS_ERR_BAD_SHAPE, MCS_ERR_BAD_HEAD_DIM, MCS_ERR_BAD_DTYPE, MCS_ERR_BAD_ALIGNMENT = -1, -2, -3, -4, -5
@@ -34,6 +35,7 @@ EXPORTED_SYMBOLS = (
     "mcs_ulysses_scatter",
     "mcs_ulysses_scatter_dma",
     "mcs_qkv_norm_rope_scatter",
+    "mcs_rotary",
     "mcs_group_mass",
     "mcs_topk_select",
     "mcs_topk_select_var",
@@ -83,6 +85,20 @@ class QkvEpilogueArgs(C.Structure):
         ("src_row_stride", C.c_int64), ("rows", C.c_int64), ("row0", C.c_int64), ("token0", C.c_int64),
         ("n_seg", C.c_int32), ("D", C.c_int32), ("grid_f", C.c_int32), ("grid_h", C.c_int32), ("grid_w", C.c_int32),
         ("pairs_t", C.c_int32), ("pairs_h", C.c_int32), ("dtype", C.c_int32), ("eps", C.c_float),
+    ]
+
+
+class RotaryArgs(C.Structure):
+    """Mirror of ``mcs_rotary_args``."""
+
+    _fields_ = [
+        ("x", C.c_void_p * 2), ("y", C.c_void_p * 2),
+        ("x_stride", (C.c_int64 * 3) * 2), ("y_stride", (C.c_int64 * 3) * 2),
+        ("positions", C.c_void_p), ("p_stride", C.c_int64 * 3),
+        ("turns", C.POINTER(C.c_uint64)), ("axis", C.POINTER(C.c_uint8)),
+        ("H", C.c_int32 * 2), ("B", C.c_int32), ("L", C.c_int32), ("D", C.c_int32),
+        ("n_pairs", C.c_int32), ("n_axes", C.c_int32), ("layout", C.c_int32), ("pos64", C.c_int32),
+        ("inverse", C.c_int32), ("dtype", C.c_int32), ("magnitude", C.c_float),
     ]
 
 
@@ -145,6 +161,8 @@ def lib() -> C.CDLL:
     L.mcs_ulysses_scatter_dma.argtypes = L.mcs_ulysses_scatter.argtypes
     L.mcs_qkv_norm_rope_scatter.restype = C.c_int
     L.mcs_qkv_norm_rope_scatter.argtypes = [C.POINTER(QkvEpilogueArgs), C.c_void_p]
+    L.mcs_rotary.restype = C.c_int
+    L.mcs_rotary.argtypes = [C.POINTER(RotaryArgs), C.c_void_p]
     L.mcs_set_clock_buffer.restype = None
     L.mcs_set_clock_buffer.argtypes = [C.c_void_p]
     L.mcs_gather_rate_probe.restype = C.c_int

@@ -375,4 +375,36 @@ int mcs_perm_invert(const void* x, void* out, const int64_t* perm, int32_t BH, i
   return perm_rows(x, out, perm, BH, L, row_bytes, x_bh, x_row, o_bh, o_row, true, stream);
 }
 
+int mcs_rotary(const mcs_rotary_args* a, void* stream) {
+  if (a == nullptr) return MCS_ERR_NULL_POINTER;
+  if (a->B < 0 || a->L < 0 || a->H[0] < 0 || a->H[1] < 0 || a->n_axes < 1 || a->n_axes > 3) return MCS_ERR_BAD_SHAPE;
+  if (a->D < 1 || a->n_pairs < 1 || a->n_pairs > mcs::kRotaryMaxPairs || 2LL * a->n_pairs > a->D) return MCS_ERR_BAD_HEAD_DIM;
+  if (a->layout != 0 && a->layout != 1) return MCS_ERR_UNSUPPORTED;
+  if (a->dtype != MCS_DTYPE_BF16 && a->dtype != MCS_DTYPE_FP16 && a->dtype != MCS_DTYPE_FP32) return MCS_ERR_BAD_DTYPE;
+  if (!std::isfinite(a->magnitude)) return MCS_ERR_BAD_SCALE;
+  if (a->turns == nullptr || a->axis == nullptr) return MCS_ERR_NULL_POINTER;
+  for (int i = 0; i < a->n_pairs; ++i)
+    if (a->axis[i] >= a->n_axes) return MCS_ERR_BAD_SHAPE;
+  if (a->B == 0 || a->L == 0 || (long long)a->H[0] + a->H[1] == 0) return 0;
+  if ((long long)a->H[0] + a->H[1] > 0x7fffffffLL) return MCS_ERR_TOO_LARGE;
+  const int es = a->dtype == MCS_DTYPE_FP32 ? 4 : 2;
+  mcs::RotaryParams p{};
+  for (int t = 0; t < 2; ++t) {
+    if (a->H[t] == 0) continue;
+    if (a->x[t] == nullptr || a->y[t] == nullptr) return MCS_ERR_NULL_POINTER;
+    if ((reinterpret_cast<uintptr_t>(a->x[t]) | reinterpret_cast<uintptr_t>(a->y[t])) % es) return MCS_ERR_BAD_ALIGNMENT;
+    p.x[t] = a->x[t]; p.y[t] = a->y[t]; p.H[t] = a->H[t];
+    for (int i = 0; i < 3; ++i) { p.x_stride[t][i] = a->x_stride[t][i]; p.y_stride[t][i] = a->y_stride[t][i]; }
+  }
+  if (a->positions == nullptr) return MCS_ERR_NULL_POINTER;
+  if (reinterpret_cast<uintptr_t>(a->positions) % (a->pos64 ? 8 : 4)) return MCS_ERR_BAD_ALIGNMENT;
+  p.positions = a->positions;
+  for (int i = 0; i < 3; ++i) p.p_stride[i] = a->p_stride[i];
+  for (int i = 0; i < a->n_pairs; ++i) { p.turns[i] = a->turns[i]; p.axis[i] = a->axis[i]; }
+  p.B = a->B; p.L = a->L; p.D = a->D; p.n_pairs = a->n_pairs;
+  p.pos64 = a->pos64 ? 1 : 0; p.inverse = a->inverse ? 1 : 0; p.magnitude = a->magnitude;
+  const int type = a->dtype == MCS_DTYPE_BF16 ? 0 : (a->dtype == MCS_DTYPE_FP16 ? 1 : 2);
+  return mcs::launch_rotary(p, type, a->layout == 1, static_cast<cudaStream_t>(stream));
+}
+
 }  // extern "C"

@@ -154,6 +154,23 @@ struct QkvEpilogueParams {
 int launch_qkv_epilogue(const QkvEpilogueParams& p, void* const* dst, const long long* dst_row_stride, const int* kind,
                         bool fp16, cudaStream_t stream);
 
+// Rotary positions of one or two tensors (rotary.cu); the plan travels in the launch's arguments
+constexpr int kRotaryMaxPairs = 128;
+struct RotaryParams {
+  const void* x[2];
+  void* y[2];
+  long long x_stride[2][3], y_stride[2][3];   // batch, row, head (elements)
+  int H[2];
+  const void* positions;
+  long long p_stride[3];                      // batch, row, axis (elements)
+  unsigned long long turns[kRotaryMaxPairs];  // part of a turn per step of position, times 2^64
+  unsigned char axis[kRotaryMaxPairs];
+  int B, L, D, n_pairs, pos64, inverse;
+  float magnitude;
+  int units, rot_units, heads_per_chunk, head_chunks;   // set by the launch
+};
+int launch_rotary(RotaryParams& p, int type, bool half, cudaStream_t stream);
+
 // Sequence-to-head reshard by peer stores (see reshard.cu)
 int launch_ulysses_scatter_dma(const void* src, void* const* dst_peers, int n_peers, int rank, long long rows,
                                long long seg_bytes, long long seg_stride_bytes, long long src_row_bytes, cudaStream_t stream);

@@ -1,0 +1,115 @@
+"""CPU tests of the rotary plan: frequencies, fixed-point turns, refusals of the wrapper and of the C entry point."""
+
+import ctypes as C
+import math
+
+import pytest
+import torch
+
+from mcsparse_b200 import _lib
+from mcsparse_b200.h3.ulysses_layer import rope_pairs
+from mcsparse_b200.kernels.flash_mcsa.ops.rotary import RotaryEmbedding
+
+
+def test_turns_are_frequencies_in_fixed_point():
+    plan = RotaryEmbedding(128, axis_pairs=rope_pairs(128))
+    assert plan.axis_pairs == (22, 21, 21) and len(plan._turns) == 64 and max(plan.pair_axis) == 2
+    for t, f in zip(plan._turns, plan.frequencies):
+        # both sides rounded once to 53 bits
+        assert abs(t / 2 ** 64 - f / (2 * math.pi)) <= 2 ** -52 * f
+    # a frequency of several turns per position keeps its part of a turn
+    from mcsparse_b200.kernels.flash_mcsa.ops.rotary import _turns
+    assert abs(_turns(10.0) / 2 ** 64 - (10.0 / (2 * math.pi)) % 1.0) < 1e-15
+    # the integer product is the angle modulo one turn, far positions and negative ones included
+    for pos in (1, 77, 10 ** 6, 2 ** 31 - 1, -5, -(2 ** 31)):
+        turn = (pos * plan._turns[0]) % 2 ** 64 / 2 ** 64
+        assert abs(math.cos(2 * math.pi * turn) - math.cos(float(pos))) < 1e-8
+
+
+def test_scalings():
+    base = RotaryEmbedding(64).frequencies
+    n = 32
+    assert base[0] == 1.0 and base[-1] == pytest.approx(10000.0 ** (-(n - 1) / n), rel=1e-14)
+    linear = RotaryEmbedding(64, scaling="linear", factor=4.0).frequencies
+    assert all(a == pytest.approx(b / 4.0, rel=1e-14) for a, b in zip(linear, base))
+    ntk = RotaryEmbedding(64, scaling="ntk", factor=4.0).frequencies
+    assert ntk[0] == 1.0
+    # the lowest frequency, i = n - 1: theta'^-(n-1)/n = theta^-(n-1)/n * factor^-1
+    assert ntk[-1] == pytest.approx(base[-1] / 4.0, rel=1e-12)
+    yarn = RotaryEmbedding(64, scaling="yarn", factor=4.0, original_length=4096)
+    turns = [4096 * f / (2 * math.pi) for f in base]
+    for f, b, r in zip(yarn.frequencies, base, turns):
+        if r >= 32:
+            assert f == b
+        elif r <= 1:
+            assert f == pytest.approx(b / 4.0, rel=1e-14)
+        else:
+            assert b / 4.0 < f < b
+    assert yarn.magnitude == pytest.approx(0.1 * math.log(4.0) + 1.0)
+    assert RotaryEmbedding(64, scaling="yarn", factor=0.5, original_length=4096).magnitude == 1.0
+    per_axis = RotaryEmbedding(128, axis_pairs=(22, 21, 21), scaling="linear", factor=(2.0, 1.0, 1.0))
+    plain = RotaryEmbedding(128, axis_pairs=(22, 21, 21))
+    assert per_axis.frequencies[0] == 0.5 and per_axis.frequencies[22:] == plain.frequencies[22:]
+
+
+@pytest.mark.parametrize("kw", [dict(rotary_dim=7), dict(rotary_dim=66), dict(rotary_dim=0), dict(axis_pairs=(10, 10)), dict(axis_pairs=(8, 8, 8, 8)),
+                                dict(axis_pairs=(33, -1)), dict(layout="rows"), dict(scaling="other"), dict(theta=0.0), dict(theta=float("nan")),
+                                dict(scaling="linear", factor=0.0), dict(scaling="linear", factor=(1.0, 2.0)),
+                                dict(scaling="yarn", factor=2.0), dict(scaling="yarn", original_length=10, beta_fast=1.0),
+                                dict(magnitude=float("inf"))])
+def test_plan_refusals(kw):
+    with pytest.raises(ValueError):
+        RotaryEmbedding(64, **kw)
+
+
+def test_call_refusals():
+    plan, grid = RotaryEmbedding(64), RotaryEmbedding(64, axis_pairs=(12, 10, 10))
+    x, pos = torch.zeros(2, 5, 3, 64), torch.arange(5)
+    bad = [
+        (ValueError, plan, (x[0],), pos), (ValueError, plan, (x[..., :32],), pos), (ValueError, plan, (x, x, x), pos),
+        (ValueError, plan, (), pos), (ValueError, plan, (x, x[:, :4]), pos), (TypeError, plan, (x.double(),), pos),
+        (TypeError, plan, (x, x.half()), pos), (TypeError, plan, (x,), pos.float()), (ValueError, plan, (x,), pos[:4]),
+        (ValueError, plan, (x,), pos.view(1, 1, 5)), (ValueError, plan, (x,), torch.zeros(3, 5, dtype=torch.int64)),
+        (ValueError, grid, (x,), pos), (ValueError, grid, (x,), torch.zeros(5, 2, dtype=torch.int64)),
+        (RuntimeError, plan, (x,), pos), (RuntimeError, grid, (x,), torch.zeros(2, 5, 3, dtype=torch.int32)),
+    ]
+    for err, p, tensors, positions in bad:
+        with pytest.raises(err):
+            p.rotate(*tensors, positions=positions)
+        with pytest.raises(err):
+            p.rotate_backward(*tensors, positions=positions)
+    with pytest.raises(RuntimeError):                       # in place is forward-only
+        plan.rotate(x.clone().requires_grad_(True), positions=pos, inplace=True)
+
+
+def test_entry_point_refusals():
+    """Validation happens before any CUDA call: the addresses below are never touched."""
+    lib = _lib.lib()
+    assert lib.mcs_rotary(None, None) == -1
+    turns, axis = (C.c_uint64 * 32)(), (C.c_uint8 * 32)()
+
+    def args(**kw):
+        a = _lib.RotaryArgs()
+        a.x[0] = a.y[0] = 0x1000
+        a.positions, a.turns, a.axis = 0x1000, turns, axis
+        a.H[0], a.B, a.L, a.D, a.n_pairs, a.n_axes, a.magnitude, a.pos64 = 4, 1, 8, 64, 32, 1, 1.0, 1
+        for k, v in kw.items():
+            setattr(a, k, v)
+        return a
+    for code, kw in [(-2, dict(B=-1)), (-2, dict(n_axes=0)), (-2, dict(n_axes=4)), (-3, dict(n_pairs=0)), (-3, dict(n_pairs=33)), (-3, dict(D=0)),
+                     (-3, dict(n_pairs=129, D=300)), (-9, dict(layout=2)), (-4, dict(dtype=2)), (-6, dict(magnitude=float("nan"))),
+                     (-1, dict(positions=None)), (-5, dict(positions=0x1004)), (0, dict(L=0)), (0, dict(B=0))]:
+        assert lib.mcs_rotary(args(**kw), None) == code, kw
+    a = args()
+    a.x[0] = None
+    assert lib.mcs_rotary(a, None) == -1
+    a = args()
+    a.x[0] = 0x1001
+    assert lib.mcs_rotary(a, None) == -5
+    a = args()
+    axis[3] = 1
+    assert lib.mcs_rotary(a, None) == -2                    # a pair on an axis that does not exist
+    axis[3] = 0
+    a = args()
+    a.H[0] = 0
+    assert lib.mcs_rotary(a, None) == 0
