@@ -204,6 +204,46 @@ typedef struct mcs_qkv_epilogue_args {
 int mcs_qkv_norm_rope_scatter(const mcs_qkv_epilogue_args* args, void* stream);
 
 /*
+ * Backward pass of the dense attention (mcs_dense_attn_fwd without perm, residual): for the gradient dout of its output,
+ *   P = exp(scale q k^T - lse), dS = P o (dout v^T - rowsum(dout o out)),
+ *   dv = P^T dout, dq = scale dS k, dk = scale dS^T q,
+ * with out and lse of the forward pass (a row with lse = -inf has no gradient).  P and dS are rounded to the inputs' type as
+ * operands of the products; all sums are fp32 and are added in a fixed order: results are bit-equal from run to run.
+ * With a single key dq and dk are exactly zero.  workspace: mcs_dense_attn_bwd_workspace_bytes(args) bytes of device memory,
+ * 256-byte aligned.  k, v, q and dout need strides that nest without overlap (else MCS_ERR_UNSUPPORTED).
+ *
+ * The reference is forward-only (mcsparse/kernels/flash_mcsa/ops/flash_sparse_attn/cute/interface.py:108-340 rejects inputs
+ * that require gradients); these entry points give the calls it makes their gradients.
+ */
+typedef struct mcs_attn_bwd_args {
+  const void* q;        /* (B, Sq, H, D), element strides below (batch, sequence, head), last dimension contiguous */
+  const void* k;        /* (B, Sk, H, D) */
+  const void* v;        /* (B, Sk, H, D) */
+  const void* out;      /* (B, Sq, H, D) of the forward pass, without residual */
+  const void* dout;     /* (B, Sq, H, D) */
+  const float* lse;     /* (B, H, Sq) contiguous fp32 of the forward pass */
+  void* dq;
+  void* dk;
+  void* dv;
+  const int32_t* gi;    /* gather only: as in mcs_gather_attn_args */
+  const int32_t* gl;    /* gather only, or NULL */
+  const int64_t* perm;  /* gather only, or NULL */
+  void* workspace;
+  int64_t workspace_bytes;
+  int32_t* status;
+  int64_t q_stride[3], k_stride[3], v_stride[3], out_stride[3], dout_stride[3], dq_stride[3], dk_stride[3], dv_stride[3];
+  int32_t B, Sq, Sk, H, D;    /* D: a multiple of 8 up to 256 */
+  int32_t gather_len;   /* gather only: multiple of 128 */
+  int32_t group_rows;   /* gather only: 1..128 */
+  int32_t dtype;        /* MCS_DTYPE_BF16 or MCS_DTYPE_FP16 */
+  float softmax_scale;  /* > 0 */
+  int32_t flags;        /* 0 */
+} mcs_attn_bwd_args;
+
+int mcs_dense_attn_bwd(const mcs_attn_bwd_args* args, void* stream);
+int64_t mcs_dense_attn_bwd_workspace_bytes(const mcs_attn_bwd_args* args);
+
+/*
  * Rotary positions of one or two (B, L, H, D) tensors in one launch (q and k of a layer): rotation pair p of every row turns by
  * w = position[axis[p]] * f_p, times a magnitude m,
  *   y_a = m (x_a cos w - x_b sin w),  y_b = m (x_a sin w + x_b cos w),

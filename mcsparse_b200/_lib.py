@@ -36,6 +36,8 @@ EXPORTED_SYMBOLS = (
     "mcs_ulysses_scatter_dma",
     "mcs_qkv_norm_rope_scatter",
     "mcs_rotary",
+    "mcs_dense_attn_bwd",
+    "mcs_dense_attn_bwd_workspace_bytes",
     "mcs_group_mass",
     "mcs_topk_select",
     "mcs_topk_select_var",
@@ -85,6 +87,22 @@ class QkvEpilogueArgs(C.Structure):
         ("src_row_stride", C.c_int64), ("rows", C.c_int64), ("row0", C.c_int64), ("token0", C.c_int64),
         ("n_seg", C.c_int32), ("D", C.c_int32), ("grid_f", C.c_int32), ("grid_h", C.c_int32), ("grid_w", C.c_int32),
         ("pairs_t", C.c_int32), ("pairs_h", C.c_int32), ("dtype", C.c_int32), ("eps", C.c_float),
+    ]
+
+
+class AttnBwdArgs(C.Structure):
+    """Mirror of ``mcs_attn_bwd_args``."""
+
+    _fields_ = [
+        ("q", C.c_void_p), ("k", C.c_void_p), ("v", C.c_void_p), ("out", C.c_void_p), ("dout", C.c_void_p),
+        ("lse", C.c_void_p), ("dq", C.c_void_p), ("dk", C.c_void_p), ("dv", C.c_void_p),
+        ("gi", C.c_void_p), ("gl", C.c_void_p), ("perm", C.c_void_p),
+        ("workspace", C.c_void_p), ("workspace_bytes", C.c_int64), ("status", C.c_void_p),
+        ("q_stride", C.c_int64 * 3), ("k_stride", C.c_int64 * 3), ("v_stride", C.c_int64 * 3), ("out_stride", C.c_int64 * 3),
+        ("dout_stride", C.c_int64 * 3), ("dq_stride", C.c_int64 * 3), ("dk_stride", C.c_int64 * 3), ("dv_stride", C.c_int64 * 3),
+        ("B", C.c_int32), ("Sq", C.c_int32), ("Sk", C.c_int32), ("H", C.c_int32), ("D", C.c_int32),
+        ("gather_len", C.c_int32), ("group_rows", C.c_int32), ("dtype", C.c_int32),
+        ("softmax_scale", C.c_float), ("flags", C.c_int32),
     ]
 
 
@@ -161,6 +179,10 @@ def lib() -> C.CDLL:
     L.mcs_ulysses_scatter_dma.argtypes = L.mcs_ulysses_scatter.argtypes
     L.mcs_qkv_norm_rope_scatter.restype = C.c_int
     L.mcs_qkv_norm_rope_scatter.argtypes = [C.POINTER(QkvEpilogueArgs), C.c_void_p]
+    L.mcs_dense_attn_bwd.restype = C.c_int
+    L.mcs_dense_attn_bwd.argtypes = [C.POINTER(AttnBwdArgs), C.c_void_p]
+    L.mcs_dense_attn_bwd_workspace_bytes.restype = C.c_int64
+    L.mcs_dense_attn_bwd_workspace_bytes.argtypes = [C.POINTER(AttnBwdArgs)]
     L.mcs_rotary.restype = C.c_int
     L.mcs_rotary.argtypes = [C.POINTER(RotaryArgs), C.c_void_p]
     L.mcs_set_clock_buffer.restype = None

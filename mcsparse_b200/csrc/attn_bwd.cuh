@@ -1,0 +1,82 @@
+// What the kernels of the attention's backward pass share: tile geometry, operand descriptors, the copy of a resident tile and
+// the two elementwise steps on score tiles.
+//
+//   P = exp(scale Q K^T - lse)      dV = P^T dO      dP = dO V^T      dS = P o (dP - delta)      delta = rowsum(dO o O)
+//   dQ = scale dS K                 dK = scale dS^T Q
+//
+// P is recomputed from the forward pass's log-sum-exp.  Scores, P, dP and dS are fp32 up to the one rounding of P and of dS to
+// the inputs' type that makes them operands of the next product; every sum is fp32.
+//
+// fp16 inputs: P and dS have to be fp16 operands, whose normal range ends at 2^-14.  P (at most 1) is taken times 2^14
+// (kBiasFp16, added to the exponent), and dS further times a power of two per (batch, head) that keeps the bound
+// |dS| <= 2 max|dO row| max|V row| below 2^15; the factors are taken out of the sums in the epilogue.
+#pragma once
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+
+#include "kernels.cuh"
+#include "ptx.cuh"
+
+namespace mcs {
+namespace bwd {
+
+constexpr float kBiasFp16 = 14.f;
+constexpr int kSoftmaxWarps = 8;       // warps 0-3 take the first half of a score tile's columns, 4-7 the second; lane == row
+
+// Power of two by which dS / 2^14 may be multiplied (see above), from the largest row norms; 1 for bf16.
+template <bool kFp16>
+__device__ __forceinline__ float ds_scale(const unsigned int* row_max, int bh) {
+  if constexpr (!kFp16) return 1.f;
+  const float m = 2.f * __uint_as_float(row_max[2 * bh]) * __uint_as_float(row_max[2 * bh + 1]);
+  if (!(m > 0.f) || isinf(m)) return 1.f;
+  int e;
+  frexpf(m, &e);                        // m < 2^e
+  e = 1 - e;
+  e = e < -60 ? -60 : (e > 60 ? 60 : e);
+  return ldexpf(1.f, e);
+}
+
+// Streamed tiles have TN rows, resident tiles 128; both are DB column blocks of 64 elements (128 bytes, swizzled).
+template <int DB, int TN>
+struct Geo {
+  static constexpr int kResBytes = DB * 16384;
+  static constexpr int kTileBytes = DB * TN * 128;
+  static constexpr int kHalf = TN / 2;                       // score columns of one softmax thread
+};
+
+constexpr uint32_t kDescHi = (1024u >> 4) | (1u << 14) | (2u << 29);     // SBO 1024, version 1, 128-byte swizzle
+__device__ __forceinline__ uint64_t desc_lo(uint32_t lo) { return (static_cast<uint64_t>(kDescHi) << 32) | lo; }
+__device__ __forceinline__ uint32_t lo_kmajor(uint32_t saddr) { return ((saddr & 0x3FFFFu) >> 4) | ((16u >> 4) << 16); }
+// MN-major operand: `block_bytes` from one block of 64 columns to the next
+__device__ __forceinline__ uint32_t lo_mnmajor(uint32_t saddr, uint32_t block_bytes) { return ((saddr & 0x3FFFFu) >> 4) | ((block_bytes >> 4) << 16); }
+
+// One warp copies `rows` rows (row_of(i): source row, or -1 for zeros) of D elements into a tile of column blocks of
+// block_rows rows, from tile row r0 on.  Columns from D on are zeros.
+template <int DB, typename RowOf>
+__device__ __forceinline__ void warp_copy_rows(uint32_t tile, int block_rows, int r0, int rows, int D, const uint8_t* base, size_t row_bytes,
+                                               const void* any, RowOf row_of) {
+  const int lane = threadIdx.x & 31;
+  constexpr int kChunks = DB * 8;
+  for (int rb = 0; rb < rows; rb += 32) {
+    const int mine = rb + lane < rows ? row_of(r0 + rb + lane) : -1;
+    const int n = min(32, rows - rb) * kChunks;
+#pragma unroll 4
+    for (int e = lane; e < n; e += 32) {
+      const int rl = e / kChunks, c = e % kChunks;
+      const int id = __shfl_sync(0xffffffffu, mine, rl);
+      const int r = r0 + rb + rl;
+      const uint32_t dst = tile + (c >> 3) * (block_rows * 128) + r * 128 + (((c & 7) ^ (r & 7)) << 4);
+      if (id >= 0 && c * 8 < D) cp_async16(dst, base + (size_t)id * row_bytes + c * 16);
+      else cp_async16_zfill(dst, any, 0);
+    }
+  }
+}
+
+template <bool kFp16>
+__device__ __forceinline__ uint32_t pack16(float a, float b) {
+  if constexpr (kFp16) return pack_f16x2(a, b);
+  else return pack_bf16x2(a, b);
+}
+
+}  // namespace bwd
+}  // namespace mcs

@@ -375,6 +375,64 @@ int mcs_perm_invert(const void* x, void* out, const int64_t* perm, int32_t BH, i
   return perm_rows(x, out, perm, BH, L, row_bytes, x_bh, x_row, o_bh, o_row, true, stream);
 }
 
+// Sizes, types and alignment of a backward call -> kernel parameters (0, or the error code)
+static int attn_bwd_params(const mcs_attn_bwd_args* a, bool gather, mcs::AttnBwdParams& p) {
+  if (a == nullptr) return MCS_ERR_NULL_POINTER;
+  if (a->B < 1 || a->H < 1 || a->Sq < 1 || a->Sk < 1) return MCS_ERR_BAD_SHAPE;
+  if (gather && (a->gather_len < 128 || a->gather_len % 128 != 0 || a->group_rows < 1 || a->group_rows > 128)) return MCS_ERR_BAD_SHAPE;
+  if (a->D < 8 || a->D > 256 || a->D % 8 != 0) return MCS_ERR_BAD_HEAD_DIM;
+  if (a->dtype != MCS_DTYPE_BF16 && a->dtype != MCS_DTYPE_FP16) return MCS_ERR_BAD_DTYPE;
+  if (!(a->softmax_scale > 0.f) || !std::isfinite(a->softmax_scale)) return MCS_ERR_BAD_SCALE;
+  if (a->flags != 0) return MCS_ERR_UNSUPPORTED;
+  if (!gather && (a->gi != nullptr || a->gl != nullptr || a->perm != nullptr)) return MCS_ERR_UNSUPPORTED;
+  const long long rows = gather ? a->group_rows : 128, tiles = ((long long)a->Sq + rows - 1) / rows, bh = (long long)a->B * a->H;
+  // work items, each split 32 times at most, and blocks of 65,535 heads of the statistics are counted in 32 bits
+  if (bh > 65535 || bh * tiles * 32 > 0x7fffffffLL || bh * (((long long)a->Sk + 127) / 128) * 64 > 0x7fffffffLL || tiles * 128 + a->Sk > 0x7fffffffLL)
+    return MCS_ERR_TOO_LARGE;
+  p.B = a->B; p.H = a->H; p.Sq = a->Sq; p.Sk = a->Sk; p.D = a->D;
+  p.gather_len = a->gather_len; p.group_rows = (int)rows; p.M = (int)tiles;
+  p.scale = a->softmax_scale; p.scale_log2 = a->softmax_scale * 1.4426950408889634f;
+  // softmax over a single key does not depend on the scores
+  p.out_scale = (!gather && a->Sk == 1) ? 0.f : a->softmax_scale;
+  p.splits = 1;
+  return 0;
+}
+
+static int attn_bwd_dispatch(const mcs_attn_bwd_args* a, bool gather, void* stream) {
+  mcs::AttnBwdParams p{};
+  const int rc = attn_bwd_params(a, gather, p);
+  if (rc != 0) return rc;
+  if (a->q == nullptr || a->k == nullptr || a->v == nullptr || a->out == nullptr || a->dout == nullptr || a->lse == nullptr || a->dq == nullptr ||
+      a->dk == nullptr || a->dv == nullptr || a->workspace == nullptr || a->status == nullptr || (gather && a->gi == nullptr))
+    return MCS_ERR_NULL_POINTER;
+  const void* ptrs[8] = {a->q, a->k, a->v, a->out, a->dout, a->dq, a->dk, a->dv};
+  const int64_t* strides[8] = {a->q_stride, a->k_stride, a->v_stride, a->out_stride, a->dout_stride, a->dq_stride, a->dk_stride, a->dv_stride};
+  for (int i = 0; i < 8; ++i) {
+    if (!aligned16(ptrs[i])) return MCS_ERR_BAD_ALIGNMENT;
+    for (int j = 0; j < 3; ++j)
+      if (strides[i][j] % 8) return MCS_ERR_BAD_ALIGNMENT;
+  }
+  if (reinterpret_cast<uintptr_t>(a->workspace) % 256) return MCS_ERR_BAD_ALIGNMENT;
+  const bool fp16 = a->dtype == MCS_DTYPE_FP16;
+  if (mcs::attn_bwd_workspace_bytes(p, gather, fp16) > a->workspace_bytes) return MCS_ERR_WORKSPACE_TOO_SMALL;
+  p.q = a->q; p.k = a->k; p.v = a->v; p.out = a->out; p.dout = a->dout; p.lse = a->lse;
+  p.dq = a->dq; p.dk = a->dk; p.dv = a->dv;
+  p.gi = a->gi; p.gl = a->gl; p.perm = a->perm; p.status = a->status;
+  for (int j = 0; j < 3; ++j) {
+    p.q_stride[j] = a->q_stride[j]; p.k_stride[j] = a->k_stride[j]; p.v_stride[j] = a->v_stride[j]; p.out_stride[j] = a->out_stride[j];
+    p.dout_stride[j] = a->dout_stride[j]; p.dq_stride[j] = a->dq_stride[j]; p.dk_stride[j] = a->dk_stride[j]; p.dv_stride[j] = a->dv_stride[j];
+  }
+  return mcs::launch_attn_bwd(p, gather, fp16, a->workspace, static_cast<cudaStream_t>(stream));
+}
+
+int mcs_dense_attn_bwd(const mcs_attn_bwd_args* a, void* stream) { return attn_bwd_dispatch(a, false, stream); }
+
+int64_t mcs_dense_attn_bwd_workspace_bytes(const mcs_attn_bwd_args* a) {
+  mcs::AttnBwdParams p{};
+  const int rc = attn_bwd_params(a, false, p);
+  return rc != 0 ? rc : mcs::attn_bwd_workspace_bytes(p, false, a->dtype == MCS_DTYPE_FP16);
+}
+
 int mcs_rotary(const mcs_rotary_args* a, void* stream) {
   if (a == nullptr) return MCS_ERR_NULL_POINTER;
   if (a->B < 0 || a->L < 0 || a->H[0] < 0 || a->H[1] < 0 || a->n_axes < 1 || a->n_axes > 3) return MCS_ERR_BAD_SHAPE;

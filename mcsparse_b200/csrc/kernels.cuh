@@ -49,7 +49,7 @@ struct alignas(64) DenseTileMaps {
 // head}; box = 64 elements x 128 rows, 128-byte swizzle.  `out` receives the 128-byte map, pos_* the coordinate
 // positions (1..3) of head, row and batch.  False if the layout cannot be described or the driver has no encoder.
 bool encode_tile_map(const void* base, const int64_t* stride, int B, int S, int H, int D, unsigned long long* out,
-                     int& pos_h, int& pos_row, int& pos_b);
+                     int& pos_h, int& pos_row, int& pos_b, int box_rows = 128);
 
 // Tensor map of K for the group-mass kernel (see DenseTileMaps)
 struct alignas(64) KeyTileMap {
@@ -170,6 +170,32 @@ struct RotaryParams {
   int units, rot_units, heads_per_chunk, head_chunks;   // set by the launch
 };
 int launch_rotary(RotaryParams& p, int type, bool half, cudaStream_t stream);
+
+// Backward pass of the dense and of the gather-KV attention (attn_bwd.cu, attn_bwd_gather.cu)
+struct AttnBwdParams {
+  const void *q, *k, *v, *out, *dout;         // (B, S, H, D), element strides {batch, row, head}
+  void *dq, *dk, *dv;
+  const float* lse;                           // (B*H, Sq) natural log
+  const int32_t *gi, *gl;                     // gather: (B*H, M, gather_len), (B*H, M) or null
+  const int64_t* perm;                        // (B*H, Sq) or null
+  int* status;
+  int64_t q_stride[3], k_stride[3], v_stride[3], out_stride[3], dout_stride[3], dq_stride[3], dk_stride[3], dv_stride[3];
+  int B, H, Sq, Sk, D;
+  int gather_len, group_rows, M;              // M query tiles of up to 128 rows (group_rows of them used)
+  float scale, scale_log2;                    // softmax scale; times log2(e)
+  float out_scale;                            // factor of dq and dk: the scale, or 0 where a single key leaves no gradient
+  // workspace
+  float *neg_lse2, *neg_delta;                // (B*H, M, 128): -(lse log2 e) (+ kBiasFp16), -rowsum(dout o out); -inf, 0 behind the last row
+  unsigned int* row_max;                      // fp16: (B*H, 2) largest norm of a row of dout, of v (as float bits)
+  float* parts;                               // split launches: partial sums
+  int splits;
+  // gather: entries that name key j of head bh lie at rows [key_start[bh][j], key_start[bh][j + 1]) of that head's block of partial
+  // sums, in the order of groups; entry_row[bh][m][slot] is the row of an entry
+  int32_t *entry_row, *key_start, *seg_count;
+  int bh0, bh_count;                          // heads of this launch
+};
+int64_t attn_bwd_workspace_bytes(const AttnBwdParams& p, bool gather, bool fp16);
+int launch_attn_bwd(AttnBwdParams& p, bool gather, bool fp16, void* workspace, cudaStream_t stream);
 
 // Sequence-to-head reshard by peer stores (see reshard.cu)
 int launch_ulysses_scatter_dma(const void* src, void* const* dst_peers, int n_peers, int rank, long long rows,

@@ -152,6 +152,11 @@ __device__ __forceinline__ void tma_load_4d(uint32_t dst, const void* tensor_map
       ::"r"(dst), "l"(tensor_map), "r"(c0), "r"(c1), "r"(c2), "r"(c3), "r"(bar)
       : "memory");
 }
+// Untiled copy of contiguous bytes into shared memory (both addresses and the size are multiples of 16 bytes).
+__device__ __forceinline__ void bulk_load(uint32_t dst, const void* src, uint32_t bytes, uint32_t bar) {
+  asm volatile("cp.async.bulk.shared::cta.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];"
+               ::"r"(dst), "l"(src), "r"(bytes), "r"(bar) : "memory");
+}
 // True in exactly one lane of a converged warp.  The MMA-issuing warps run their loops converged,
 // with warp-uniform operands, and predicate only the tcgen05 instruction itself on this: issued from
 // a lane-dependent branch instead, every operand has to be moved from per-thread to uniform registers
@@ -371,6 +376,11 @@ __device__ __forceinline__ unsigned long long f2_fma(unsigned long long a, unsig
 __device__ __forceinline__ unsigned long long f2_add(unsigned long long a, unsigned long long b) {
   unsigned long long r;
   asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ unsigned long long f2_mul(unsigned long long a, unsigned long long b) {
+  unsigned long long r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
   return r;
 }
 // Three-input maximum (one instruction on sm_100).

@@ -29,9 +29,9 @@ PFN_cuTensorMapEncodeTiled tensor_map_encoder() {
 
 // 4-D tensor map of a (B, S, H, D) tensor of 16-bit elements with element strides {batch, row, head}: D innermost,
 // then head / row / batch in the order of ascending stride (dimensions of extent 1 last, packed).  Box: 64
-// elements (128 bytes, the swizzle span) x 128 rows.  Returns false if the layout cannot be described.
+// elements (128 bytes, the swizzle span) x box_rows rows.  Returns false if the layout cannot be described.
 bool encode_tile_map(const void* base, const int64_t* stride, int B, int S, int H, int D, unsigned long long* out,
-                     int& pos_h, int& pos_row, int& pos_b) {
+                     int& pos_h, int& pos_row, int& pos_b, int box_rows) {
   PFN_cuTensorMapEncodeTiled enc = tensor_map_encoder();
   if (enc == nullptr) return false;
   struct Dim { int which; unsigned long long extent; long long stride_bytes; };
@@ -53,7 +53,7 @@ bool encode_tile_map(const void* base, const int64_t* stride, int B, int S, int 
     strides[i] = (cuuint64_t)sb;
     prev_end = (unsigned long long)sb * d[i].extent;
     if (d[i].which == 0) pos_h = i + 1;
-    if (d[i].which == 1) { pos_row = i + 1; box[i + 1] = 128; }
+    if (d[i].which == 1) { pos_row = i + 1; box[i + 1] = (cuuint32_t)box_rows; }
     if (d[i].which == 2) pos_b = i + 1;
   }
   CUtensorMap tm;

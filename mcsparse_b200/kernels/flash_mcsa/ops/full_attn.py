@@ -77,3 +77,55 @@ def full_attention_with_lse(q: Tensor, k: Tensor, v: Tensor, scale: Optional[flo
     permuted, "group" order the anchor step works in) with ``group_order``."""
     out, lse = _dense(q, k, v, scale, want_lse=True, perm=perm, group_order=group_order)
     return out, lse
+
+
+def full_attention_backward(dout: Tensor, q: Tensor, k: Tensor, v: Tensor, out: Tensor, lse: Tensor,
+                            scale: Optional[float] = None) -> Tuple[Tensor, Tensor, Tensor]:
+    """Gradients (dq, dk, dv) of :func:`full_attention` for the gradient ``dout`` of its output, from ``out`` and ``lse`` as
+    :func:`full_attention_with_lse` returned them (without ``perm``) and the same ``scale``.
+
+    All tensors (B, H, L, D), bf16 or fp16, head dimension a multiple of 8 up to 256, lengths of q and k independent; each
+    gradient has its tensor's layout where that one's rows are contiguous.  Probabilities are recomputed from ``lse``, sums are
+    fp32 in a fixed order: the same inputs give the same bits.  (The reference is forward-only.)"""
+    from mcsparse_b200.kernels.flash_mcsa.ops import attn_bwd
+    if q.dim() != 4 or k.dim() != 4 or k.shape != v.shape or q.shape[:2] != k.shape[:2] or q.shape[3] != k.shape[3]:
+        raise ValueError(f"expected (B, H, L, D) tensors, got q {tuple(q.shape)}, k {tuple(k.shape)}, v {tuple(v.shape)}")
+    if q.dtype not in (torch.bfloat16, torch.float16) or k.dtype != q.dtype or v.dtype != q.dtype:
+        raise TypeError("dense attention needs bf16 or fp16 q, k, v of one dtype")
+    B, H, Lq, D = q.shape
+    if D % 8 or not 8 <= D <= 256:
+        raise ValueError(f"head dimension must be a multiple of 8 up to 256, got {D}")
+    if min(B, H, Lq, k.shape[2]) < 1:
+        raise ValueError(f"every size must be at least 1, got q {tuple(q.shape)}, k {tuple(k.shape)}")
+    attn_bwd.check_saved(dout, out, lse, q, (B, H, Lq))
+    if scale is None:
+        scale = 1.0 / math.sqrt(D)
+    if not q.is_cuda:
+        raise RuntimeError("dense attention runs on a CUDA device only; there is no CPU path")
+    if k.device != q.device or v.device != q.device:
+        raise ValueError("q, k and v must be on one device")
+    dq, dk, dv = (torch.empty_like(t) if t.stride(-1) == 1 else torch.empty(t.shape, dtype=t.dtype, device=t.device) for t in (q, k, v))
+    dov, qv, kv, vv, ov = (attn_bwd.readable(t.detach().transpose(1, 2)) for t in (dout, q, k, v, out))
+    attn_bwd.launch_backward("mcs_dense_attn_bwd", dov, qv, kv, vv, ov, lse.detach().contiguous(), dq.transpose(1, 2), dk.transpose(1, 2),
+                             dv.transpose(1, 2), scale)
+    return dq, dk, dv
+
+
+class _FullAttention(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, q: Tensor, k: Tensor, v: Tensor, scale: Optional[float]):
+        q, k, v = q.detach(), k.detach(), v.detach()
+        out, lse = full_attention_with_lse(q, k, v, scale)
+        ctx.save_for_backward(q, k, v, out, lse)
+        ctx.scale = scale
+        return out
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dout: Tensor):
+        return (*full_attention_backward(dout, *ctx.saved_tensors, scale=ctx.scale), None)
+
+
+def full_attention_autograd(q: Tensor, k: Tensor, v: Tensor, scale: Optional[float] = None) -> Tensor:
+    """:func:`full_attention` that autograd can differentiate (once) in q, k and v; same values."""
+    return _FullAttention.apply(q, k, v, scale)
