@@ -78,5 +78,24 @@ __device__ __forceinline__ uint32_t pack16(float a, float b) {
   else return pack_bf16x2(a, b);
 }
 
+// two 16-bit values as packed fp32
+template <bool kFp16>
+__device__ __forceinline__ unsigned long long unpack16(uint32_t u) {
+  if constexpr (kFp16) {
+    const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&u));
+    return f2_pack(f.x, f.y);
+  } else {
+    return f2_pack(bf16_lo(u), bf16_hi(u));
+  }
+}
+// sixteen fp32 values, rounded, into eight tensor-memory columns of this thread's lane
+template <bool kFp16>
+__device__ __forceinline__ void store_packed(uint32_t taddr, const uint32_t* v) {
+  uint32_t pk[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) pk[i] = pack16<kFp16>(__uint_as_float(v[2 * i]), __uint_as_float(v[2 * i + 1]));
+  tmem_st8(taddr, pk);
+}
+
 }  // namespace bwd
 }  // namespace mcs

@@ -12,6 +12,8 @@ with fp32 products and sums, P and dS rounded once to the input type (relative s
 * dS: u |dS| from the rounding of the operand; err(P) |dP - delta|; P times the error of dP, 2^-20 |dO||V|^T, and of delta: the
   difference that the given (rounded) `out` makes, which is computed here, and 2^-20 sum|dO||out|; its products with |K|, |Q| are
   summed;  sums in fp32 add 2^-20 of the sums of magnitudes;
+* dQ: the kernel subtracts r PK, r the sum of a row's rounded dS (zero but for the errors above, so |r| is at most their sum) and
+  PK = P K: beside sum err(dS) |K| at most sum err(dS) times P |K|;
 * fp16: P and dS are scaled by powers of two such that the half-step of the smallest fp16 numbers, 2^-25, stands for less than
   2^-39 of P's largest value 1 and of the bound 2 max|dO| max|V| of dS;
 * the result's own rounding, u of its value.
@@ -45,7 +47,8 @@ def head_grads(q, k, v, dout, out, scale, dtype, hide=None):
     if dtype == torch.float16:
         err_dv = err_dv + 2.0 ** -39
         err_ds = err_ds + 2.0 ** -39 * 2 * dout.norm(dim=-1).max() * v.norm(dim=-1).max()
-    tol_dq, tol_dk = scale * err_ds @ k.abs(), scale * err_ds.t() @ q.abs()
+    tol_dq = scale * (err_ds @ k.abs() + err_ds.sum(-1, keepdim=True) * (p @ k.abs()))
+    tol_dk = scale * err_ds.t() @ q.abs()
     return (dq, dk, dv), (tol_dq, tol_dk, err_dv.t() @ dout.abs())
 
 
