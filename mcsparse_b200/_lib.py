@@ -38,6 +38,8 @@ EXPORTED_SYMBOLS = (
     "mcs_rotary",
     "mcs_dense_attn_bwd",
     "mcs_dense_attn_bwd_workspace_bytes",
+    "mcs_gather_attn_bwd",
+    "mcs_gather_attn_bwd_workspace_bytes",
     "mcs_group_mass",
     "mcs_topk_select",
     "mcs_topk_select_var",
@@ -179,10 +181,9 @@ def lib() -> C.CDLL:
     L.mcs_ulysses_scatter_dma.argtypes = L.mcs_ulysses_scatter.argtypes
     L.mcs_qkv_norm_rope_scatter.restype = C.c_int
     L.mcs_qkv_norm_rope_scatter.argtypes = [C.POINTER(QkvEpilogueArgs), C.c_void_p]
-    L.mcs_dense_attn_bwd.restype = C.c_int
-    L.mcs_dense_attn_bwd.argtypes = [C.POINTER(AttnBwdArgs), C.c_void_p]
-    L.mcs_dense_attn_bwd_workspace_bytes.restype = C.c_int64
-    L.mcs_dense_attn_bwd_workspace_bytes.argtypes = [C.POINTER(AttnBwdArgs)]
+    for fn, size in ((L.mcs_dense_attn_bwd, L.mcs_dense_attn_bwd_workspace_bytes), (L.mcs_gather_attn_bwd, L.mcs_gather_attn_bwd_workspace_bytes)):
+        fn.restype, size.restype = C.c_int, C.c_int64
+        fn.argtypes, size.argtypes = [C.POINTER(AttnBwdArgs), C.c_void_p], [C.POINTER(AttnBwdArgs)]
     L.mcs_rotary.restype = C.c_int
     L.mcs_rotary.argtypes = [C.POINTER(RotaryArgs), C.c_void_p]
     L.mcs_set_clock_buffer.restype = None

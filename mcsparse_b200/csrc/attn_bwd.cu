@@ -639,7 +639,11 @@ int pick_splits(long long items, int T, int sms) {
   return pick;
 }
 
-struct Plan { int dq_splits, kv_splits; size_t stats, row_max, parts, total; };
+// Most bytes of one pass's contributions in the gather call (a single head's may be more).  They pass through DRAM anyway; smaller
+// passes would only add launches with a partly filled last wave.
+constexpr size_t kPartsBytes = 4ull << 30;
+
+struct Plan { int dq_splits, kv_splits, segs, heads_per_pass; size_t stats, row_max, entries, starts, counts, parts, total; };
 
 constexpr size_t kAlign = 256;
 size_t up(size_t n) { return (n + kAlign - 1) / kAlign * kAlign; }
@@ -659,7 +663,23 @@ Plan make_plan(const AttnBwdParams& p, bool gather) {
   w.row_max = up((size_t)bh * 8);
   size_t a = w.dq_splits > 1 ? (size_t)w.dq_splits * bh * p.Sq * (2 * p.D + 8) * 4 : 0, b = w.kv_splits > 1 ? (size_t)w.kv_splits * bh * p.Sk * 2 * p.D * 4 : 0;
   w.parts = up(a > b ? a : b);
-  w.total = 2 * w.stats + w.row_max + w.parts;
+  if (gather) {
+    // segments of groups: enough CTAs for the counting sort without counts that outgrow the indices
+    const long long want = (4 * kSms + bh - 1) / bh;
+    w.segs = (int)(want < 16 ? want : 16);
+    if (w.segs > p.M) w.segs = p.M;
+    w.entries = up((size_t)bh * p.M * p.gather_len * 4);
+    w.starts = up((size_t)bh * (p.Sk + 1) * 4);
+    w.counts = up((size_t)bh * w.segs * p.Sk * 4);
+    // the contributions of as many heads at a time as fit kPartsBytes, at least one
+    const size_t head = (size_t)p.M * p.gather_len * 2 * p.D * 4;
+    const long long fit = (long long)(kPartsBytes / head);
+    w.heads_per_pass = (int)(fit < 1 ? 1 : (fit > bh ? bh : fit));
+    const int passes = (int)((bh + w.heads_per_pass - 1) / w.heads_per_pass);
+    w.heads_per_pass = (int)((bh + passes - 1) / passes);
+    w.parts = up(w.heads_per_pass * head);
+  }
+  w.total = 2 * w.stats + w.row_max + w.entries + w.starts + w.counts + w.parts;
   return w;
 }
 
@@ -703,12 +723,29 @@ int launch_dense(AttnBwdParams& p, const Plan& w, cudaStream_t stream) {
   return cudaGetLastError() == cudaSuccess ? 0 : -8;
 }
 
+template <int DB, int TN, bool kFp16>
+int launch_gather_dq(AttnBwdParams& p, cudaStream_t stream) {
+  auto dq = attn_bwd_kernel<DB, TN, kFp16, kDqGather>;
+  constexpr int kSmem = SmemB<DB, TN>::kDynamic;
+  if (set_smem(dq, kSmem)) return -8;
+  const int sms = sm_count();
+  p.splits = 1;
+  const long long items = (long long)p.B * p.H * p.M * column_blocks(p.D);
+  dq<<<(unsigned)(items < sms ? items : sms), 480, kSmem, stream>>>(p, DenseTileMaps{});
+  return cudaGetLastError() == cudaSuccess ? 0 : -8;
+}
+
 template <bool kFp16>
-int launch_type(AttnBwdParams& p, const Plan& w, cudaStream_t stream) {
+int launch_type(AttnBwdParams& p, const Plan& w, bool gather, cudaStream_t stream) {
   if (kFp16 && cudaMemsetAsync(p.row_max, 0, (size_t)p.B * p.H * 8, stream) != cudaSuccess) return -8;
   const int rows = p.M * 128 + (kFp16 ? p.Sk : 0);
   const int per = (rows + 15) / 16;
   attn_bwd_stats_kernel<kFp16><<<dim3((unsigned)(per < 256 ? per : 256), (unsigned)(p.B * p.H)), 256, 0, stream>>>(p);
+  if (gather) {
+    const int db = padded_blocks(p.D);
+    const int rc = db == 1 ? launch_gather_dq<1, 128, kFp16>(p, stream) : (db == 2 ? launch_gather_dq<2, 128, kFp16>(p, stream) : launch_gather_dq<4, 64, kFp16>(p, stream));
+    return rc != 0 ? rc : launch_attn_bwd_gather_dkv(p, kFp16, w.segs, w.heads_per_pass, stream);
+  }
   switch (padded_blocks(p.D)) {
     case 1: return launch_dense<1, 128, kFp16>(p, w, stream);
     case 2: return launch_dense<2, 128, kFp16>(p, w, stream);
@@ -726,8 +763,12 @@ int launch_attn_bwd(AttnBwdParams& p, bool gather, bool fp16, void* workspace, c
   p.neg_lse2 = reinterpret_cast<float*>(ws);
   p.neg_delta = reinterpret_cast<float*>(ws + w.stats);
   p.row_max = reinterpret_cast<unsigned int*>(ws + 2 * w.stats);
-  p.parts = reinterpret_cast<float*>(ws + 2 * w.stats + w.row_max);
-  return fp16 ? launch_type<true>(p, w, stream) : launch_type<false>(p, w, stream);
+  ws += 2 * w.stats + w.row_max;
+  p.entry_row = reinterpret_cast<int32_t*>(ws);
+  p.key_start = reinterpret_cast<int32_t*>(ws + w.entries);
+  p.seg_count = reinterpret_cast<int32_t*>(ws + w.entries + w.starts);
+  p.parts = reinterpret_cast<float*>(ws + w.entries + w.starts + w.counts);
+  return fp16 ? launch_type<true>(p, w, gather, stream) : launch_type<false>(p, w, gather, stream);
 }
 
 }  // namespace mcs

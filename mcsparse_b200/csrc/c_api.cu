@@ -389,6 +389,7 @@ static int attn_bwd_params(const mcs_attn_bwd_args* a, bool gather, mcs::AttnBwd
   // work items, each split 32 times at most, and blocks of 65,535 heads of the statistics are counted in 32 bits
   if (bh > 65535 || bh * tiles * 32 > 0x7fffffffLL || bh * (((long long)a->Sk + 127) / 128) * 64 > 0x7fffffffLL || tiles * 128 + a->Sk > 0x7fffffffLL)
     return MCS_ERR_TOO_LARGE;
+  if (gather && tiles * a->gather_len > 0x7fffffffLL) return MCS_ERR_TOO_LARGE;       // rows of one head's entries are 32-bit
   p.B = a->B; p.H = a->H; p.Sq = a->Sq; p.Sk = a->Sk; p.D = a->D;
   p.gather_len = a->gather_len; p.group_rows = (int)rows; p.M = (int)tiles;
   p.scale = a->softmax_scale; p.scale_log2 = a->softmax_scale * 1.4426950408889634f;
@@ -431,6 +432,14 @@ int64_t mcs_dense_attn_bwd_workspace_bytes(const mcs_attn_bwd_args* a) {
   mcs::AttnBwdParams p{};
   const int rc = attn_bwd_params(a, false, p);
   return rc != 0 ? rc : mcs::attn_bwd_workspace_bytes(p, false, a->dtype == MCS_DTYPE_FP16);
+}
+
+int mcs_gather_attn_bwd(const mcs_attn_bwd_args* a, void* stream) { return attn_bwd_dispatch(a, true, stream); }
+
+int64_t mcs_gather_attn_bwd_workspace_bytes(const mcs_attn_bwd_args* a) {
+  mcs::AttnBwdParams p{};
+  const int rc = attn_bwd_params(a, true, p);
+  return rc != 0 ? rc : mcs::attn_bwd_workspace_bytes(p, true, a->dtype == MCS_DTYPE_FP16);
 }
 
 int mcs_rotary(const mcs_rotary_args* a, void* stream) {

@@ -454,6 +454,106 @@ def flash_attn_gather_kv_fp8_func(
     return (out, lse) if return_lse else (out, None)
 
 
+def flash_attn_gather_kv_backward_func(
+    dout: torch.Tensor,
+    q: torch.Tensor,
+    k: torch.Tensor,
+    v: torch.Tensor,
+    out: torch.Tensor,
+    lse: torch.Tensor,
+    gather_kv_indices: torch.Tensor,
+    softmax_scale: Optional[float] = None,
+    gather_kv_lengths: Optional[torch.Tensor] = None,
+    *,
+    perm: Optional[torch.Tensor] = None,
+    group_rows: int = 128,
+) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+    """Gradients (dq, dk, dv) of :func:`flash_attn_gather_kv_func` (fp16 / bf16, head dimension a multiple of 8 up to 256).
+
+    ``dout``: gradient of its output; ``out`` and ``lse``: what it returned for these arguments **without** a residual and
+    with ``return_lse=True`` (a residual is added outside and gets ``dout`` itself as its gradient, in permuted order where
+    ``perm`` is given).  Layouts, indices (int32 or :class:`PackedIndices`), lengths, ``perm`` and ``group_rows`` as in the
+    forward pass; all gradients are in the original row order.  A key's gradient sums over the groups that selected it, once
+    per entry; keys that no group selected get zeros.  Sums are fp32 in a fixed order: the same inputs give the same bits.
+
+    The contributions of up to 4 GiB at a time (at least one head's: 8 * D bytes per entry) pass through a temporary buffer.
+    (The reference is forward-only.)
+    """
+    from mcsparse_b200.kernels.flash_mcsa.ops import attn_bwd
+    if q.dtype not in (torch.float16, torch.bfloat16):
+        raise TypeError(f"q/k/v must be fp16 or bf16, got {q.dtype}")
+    if not (q.dtype == k.dtype == v.dtype):
+        raise TypeError("q, k and v must have the same dtype")
+    batch_size, seqlen_q, seqlen_k, num_head, head_dim, head_dim_v = _shape_checks(q, k, v)
+    _validate_head_dims(head_dim, head_dim_v, 8)
+    if head_dim_v != head_dim:
+        raise ValueError(f"Unsupported head_dim={head_dim}/head_dim_v={head_dim_v}: head_dim_v must equal head_dim")
+    if min(batch_size, seqlen_q, seqlen_k, num_head, head_dim) < 1:
+        raise ValueError(f"every size must be at least 1, got q {tuple(q.shape)}, k {tuple(k.shape)}")
+    if not (1 <= int(group_rows) <= 128):
+        raise ValueError(f"group_rows must be in [1, 128], got {group_rows}")
+    gather_kv_indices, gather_kv_lengths, _ = _index_checks(gather_kv_indices, gather_kv_lengths, batch_size, num_head,
+                                                            math.ceil(seqlen_q / group_rows), seqlen_k)
+    attn_bwd.check_saved(dout, out, lse, q, (batch_size, num_head, seqlen_q))
+    _, perm = _extras_checks(None, perm, q, q.dtype, batch_size, num_head, seqlen_q, head_dim_v)
+    others = [k, v] + ([gather_kv_lengths] if gather_kv_lengths is not None else [])
+    if any(t.device != q.device for t in (*others, gather_kv_indices)):
+        raise ValueError("q, k, v, gather_kv_indices and gather_kv_lengths must be on one device")
+    if not q.is_cuda:
+        raise RuntimeError("CUDA is required")
+    if _device_arch(q.device.index) // 10 != 10:
+        raise RuntimeError(f"gather-KV backward requires SM100/Blackwell (B200), got sm_{_device_arch(q.device.index)}")
+    if softmax_scale is None:
+        softmax_scale = 1.0 / math.sqrt(head_dim)
+    if isinstance(gather_kv_indices, PackedIndices):
+        with torch.cuda.device(q.device):
+            gather_kv_indices = gather_kv_indices.unpack()
+    dq, dk, dv = (torch.empty_like(t) if t.stride(-1) == 1 else torch.empty(t.shape, dtype=t.dtype, device=t.device) for t in (q, k, v))
+    dov, qv, kv, vv, ov = (attn_bwd.readable(t.detach()) for t in (dout, q, k, v, out))
+    attn_bwd.launch_backward("mcs_gather_attn_bwd", dov, qv, kv, vv, ov, lse.detach().contiguous(), dq, dk, dv, softmax_scale,
+                             gather_kv_indices, gather_kv_lengths, perm, group_rows)
+    return dq, dk, dv
+
+
+class _GatherAttention(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, q, k, v, gather_kv_indices, softmax_scale, gather_kv_lengths, perm, group_rows):
+        q, k, v = q.detach(), k.detach(), v.detach()
+        out, lse = flash_attn_gather_kv_func(q, k, v, gather_kv_indices, softmax_scale=softmax_scale, return_lse=True,
+                                             gather_kv_lengths=gather_kv_lengths, perm=perm, group_rows=group_rows)
+        packed = isinstance(gather_kv_indices, PackedIndices)
+        index_tensors = (gather_kv_indices.lo, gather_kv_indices.hi) if packed else (gather_kv_indices,)
+        ctx.save_for_backward(q, k, v, out, lse, gather_kv_lengths, perm, *index_tensors)
+        ctx.index_shape = gather_kv_indices.shape if packed else None
+        ctx.softmax_scale, ctx.group_rows = softmax_scale, group_rows
+        return out
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dout):
+        q, k, v, out, lse, gl, perm, *gi = ctx.saved_tensors
+        gi = gi[0] if ctx.index_shape is None else PackedIndices(*gi, ctx.index_shape)
+        grads = flash_attn_gather_kv_backward_func(dout, q, k, v, out, lse, gi, ctx.softmax_scale, gl, perm=perm, group_rows=ctx.group_rows)
+        return (*grads, None, None, None, None, None)
+
+
+def flash_attn_gather_kv_autograd_func(
+    q: torch.Tensor,
+    k: torch.Tensor,
+    v: torch.Tensor,
+    gather_kv_indices: torch.Tensor,
+    softmax_scale: Optional[float] = None,
+    gather_kv_lengths: Optional[torch.Tensor] = None,
+    *,
+    perm: Optional[torch.Tensor] = None,
+    group_rows: int = 128,
+) -> torch.Tensor:
+    """The output of :func:`flash_attn_gather_kv_func` (same values), differentiable (once) in q, k and v.  The selection is
+    not differentiated: indices, lengths and ``perm`` are constants of the step.  They must not be overwritten before the
+    backward pass (autograd raises if they were)."""
+    return _GatherAttention.apply(q, k, v, gather_kv_indices, softmax_scale, gather_kv_lengths, perm, int(group_rows))
+
+
 def flash_attn_func(
     q: torch.Tensor,
     k: torch.Tensor,
