@@ -83,6 +83,7 @@ __global__ void __launch_bounds__(256) attn_bwd_stats_kernel(const AttnBwdParams
         }
         p.neg_lse2[(size_t)bh * rows + i] = nl;
         p.neg_delta[(size_t)bh * rows + i] = nd;
+        if (row < 0) p.neg_delta_kv[(size_t)bh * rows + i] = 0.f;      // (the others are written with dQ)
       }
       if constexpr (kFp16) m_do = fmaxf(m_do, sq);
     } else if constexpr (kFp16) {
@@ -122,7 +123,8 @@ __global__ void __launch_bounds__(256) attn_bwd_stats_kernel(const AttnBwdParams
 // dQ is off by r times the keys that a row looks at, which does not average out where these keys resemble one another (with
 // clusters of neighbouring tokens the error of dQ was 5.6e-3 of its norm in bf16, 1.7e-3 of it the result's own rounding).  The
 // kernel therefore sums the rounded dS, and PK = sum_j P_ij K_j beside dQ, and stores dQ - r PK: 2.3e-3.  The fourth product takes
-// the tensor pipe as long as the kernel of dK and dV does; r is exact where P was computed from the same scores.
+// the tensor pipe as long as the kernel of dK and dV does.  The sum of dS before rounding, too, is taken: it is what delta is off
+// by, and the key side, which runs second, gets delta without it (dK: 2.7e-3 -> 2.4e-3 with lists of selected keys).
 enum { kDq = 0, kDqGather = 1, kDkv = 2 };
 
 template <int DB, int TN>
@@ -132,7 +134,7 @@ struct SmemB {
   static constexpr int kA0 = 0, kA1 = G::kResBytes;
   static constexpr int kRingOff = 2 * G::kResBytes;
   static constexpr int kStat = kRingOff + kRing * G::kTileBytes;           // kDkv: TN floats per slot, lse2 with Q, delta with dO; kDq: sums of dS
-  static constexpr int kStatBytes = kRing * TN * 4 > 1024 ? kRing * TN * 4 : 1024;
+  static constexpr int kStatBytes = kRing * TN * 4 > 1536 ? kRing * TN * 4 : 1536;
   static constexpr int kBars = kStat + kStatBytes;
   static constexpr int kFull = 0, kEmpty = kRing, kAFull = 2 * kRing, kAEmpty = kAFull + 1, kSFull = kAEmpty + 1, kDPFull = kSFull + 1,
                        kPReady = kDPFull + 1, kDSReady = kPReady + 1, kOFull = kDSReady + 1, kOFree = kOFull + 1, kRowSum = kOFree + 1,
@@ -242,7 +244,7 @@ __global__ void __launch_bounds__(kMode == kDqGather ? 480 : 384, 1) attn_bwd_ke
       const Item it = decode(item);
       const float c = ds_scale<kFp16>(p.row_max, it.bh);
       const unsigned long long c2 = f2_pack(c, c);
-      unsigned long long nl2 = 0, nd2 = 0, rs[2] = {0, 0};   // kDq: this row's statistics, sum of its rounded dS
+      unsigned long long nl2 = 0, nd2 = 0, rs[2] = {0, 0}, es[2] = {0, 0};   // kDq: this row's statistics, sums of its dS rounded and not
       if constexpr (!kRowsAreKeys) {
         const size_t si = ((size_t)it.bh * p.M + it.m) * 128 + r_in;
         const float nl = p.neg_lse2[si], ndl = p.neg_delta[si];
@@ -320,11 +322,14 @@ __global__ void __launch_bounds__(kMode == kDqGather ? 480 : 384, 1) attn_bwd_ke
               unsigned long long d0 = f2_add(f2_pack(__uint_as_float(dp[e]), __uint_as_float(dp[e + 1])), e0);
               unsigned long long d1 = f2_add(f2_pack(__uint_as_float(dp[e + 2]), __uint_as_float(dp[e + 3])), e1);
               if constexpr (kFp16) { d0 = f2_mul(d0, c2); d1 = f2_mul(d1, c2); }
-              const float2 y0 = f2_unpack(f2_mul(f2_pack(__uint_as_float(sc[s0 + e]), __uint_as_float(sc[s0 + e + 1])), d0));
-              const float2 y1 = f2_unpack(f2_mul(f2_pack(__uint_as_float(sc[s0 + e + 2]), __uint_as_float(sc[s0 + e + 3])), d1));
+              d0 = f2_mul(f2_pack(__uint_as_float(sc[s0 + e]), __uint_as_float(sc[s0 + e + 1])), d0);
+              d1 = f2_mul(f2_pack(__uint_as_float(sc[s0 + e + 2]), __uint_as_float(sc[s0 + e + 3])), d1);
+              const float2 y0 = f2_unpack(d0), y1 = f2_unpack(d1);
               pk[2 * i] = pack16<kFp16>(y0.x, y0.y);
               pk[2 * i + 1] = pack16<kFp16>(y1.x, y1.y);
               if constexpr (!kRowsAreKeys) {
+                es[0] = f2_add(es[0], d0);
+                es[1] = f2_add(es[1], d1);
                 rs[0] = f2_add(rs[0], unpack16<kFp16>(pk[2 * i]));
                 rs[1] = f2_add(rs[1], unpack16<kFp16>(pk[2 * i + 1]));
               }
@@ -338,17 +343,23 @@ __global__ void __launch_bounds__(kMode == kDqGather ? 480 : 384, 1) attn_bwd_ke
       }
       if (!ok) break;
       const float unbias = kFp16 ? 6.103515625e-05f : 1.f;                     // 2^-14
-      float fix = 0.f;
+      float fix = 0.f, off = 0.f;
       if constexpr (!kRowsAreKeys) {
-        // the row's sum of dS from its two threads; the other's value is read before this item's kOFree, so before it is written again
+        // the row's sums of dS from its two threads; the other's are read before this item's kOFree, so before they are written again
         float* sums = reinterpret_cast<float*>(smem + L::kStat);
-        const float2 a = f2_unpack(rs[0]), b = f2_unpack(rs[1]);
-        const float mine = (a.x + a.y) + (b.x + b.y);
-        sums[x * 128 + r_in] = mine;
+        const float2 a = f2_unpack(rs[0]), b = f2_unpack(rs[1]), a2 = f2_unpack(es[0]), b2 = f2_unpack(es[1]);
+        sums[x * 128 + r_in] = (a.x + a.y) + (b.x + b.y);
+        off = (a2.x + a2.y) + (b2.x + b2.y);
+        if (x == 1) sums[256 + r_in] = off;
         warp_arrive(bar(L::kRowSum));
         ok = mbar_wait(bar(L::kRowSum), ic & 1, p.status, 134);
         if (!ok) break;
-        fix = (x == 0 ? mine + sums[128 + r_in] : sums[r_in] + mine);
+        fix = sums[r_in] + sums[128 + r_in];
+        off = (off + sums[256 + r_in]) * unbias / c;         // (used by the first half only)
+        if (p.splits == 1 && x == 0 && it.c0 == 0) {
+          const size_t si = ((size_t)it.bh * p.M + it.m) * 128 + r_in;
+          p.neg_delta_kv[si] = p.neg_delta[si] - off;
+        }
       }
       ok = mbar_wait(bar(L::kOFull), ic & 1, p.status, 135);
       if (!ok) break;
@@ -362,7 +373,7 @@ __global__ void __launch_bounds__(kMode == kDqGather ? 480 : 384, 1) attn_bwd_ke
       void* dst = kRowsAreKeys ? (second ? p.dk : p.dv) : p.dq;
       uint8_t* optr = reinterpret_cast<uint8_t*>(dst) + 2 * ((size_t)it.b * st[0] + safe * st[1] + (size_t)it.h * st[2]);
       const int S = kRowsAreKeys ? p.Sk : p.Sq;
-      // a row of partial sums: dK | dV, or dQ | PK | sum of dS (padded to 8 floats)
+      // a row of partial sums: dK | dV, or dQ | PK | the sums of dS (padded to 8 floats)
       const int pitch = kRowsAreKeys ? 2 * p.D : 2 * p.D + 8;
       float* part = p.parts + (((size_t)it.split * p.B * p.H + it.bh) * S + safe) * pitch;
       const int mid = ((it.ncol / 16 + 1) / 2) * 16;
@@ -407,7 +418,10 @@ __global__ void __launch_bounds__(kMode == kDqGather ? 480 : 384, 1) attn_bwd_ke
         }
         __syncwarp();
       }
-      if (!kRowsAreKeys && p.splits > 1 && x == 0 && row >= 0 && it.c0 == 0) part[2 * p.D] = fix * w;
+      if (!kRowsAreKeys && p.splits > 1 && x == 0 && row >= 0 && it.c0 == 0) {
+        part[2 * p.D] = fix * w;
+        part[2 * p.D + 1] = off;
+      }
       tc_fence_before();
       warp_arrive(bar(L::kOFree));
       ++ic;
@@ -564,7 +578,7 @@ __global__ void __launch_bounds__(kMode == kDqGather ? 480 : 384, 1) attn_bwd_ke
           for (int cb = 0; cb < DB; ++cb)
             tma_load_4d(sRing(slot) + cb * TN * 128, map, cb * 64, co[1], co[2], co[3], bar(L::kFull + slot));
           if constexpr (kRowsAreKeys)
-            bulk_load(s_base + L::kStat + slot * TN * 4, (is_t1 ? p.neg_delta : p.neg_lse2) + (size_t)it.bh * p.M * 128 + (size_t)(e >> 1) * TN, TN * 4,
+            bulk_load(s_base + L::kStat + slot * TN * 4, (is_t1 ? p.neg_delta_kv : p.neg_lse2) + (size_t)it.bh * p.M * 128 + (size_t)(e >> 1) * TN, TN * 4,
                       bar(L::kFull + slot));
         }
       }
@@ -586,10 +600,12 @@ __global__ void __launch_bounds__(kMode == kDqGather ? 480 : 384, 1) attn_bwd_ke
 
 // ------------------------------------------------------------------------------------------------ sums of split launches
 // parts: (splits, B*H, S, pitch) fp32; columns [col0, col0 + D) are added in the order of the splits, rounded once and stored.
-// kFix (dQ): minus the row's sum of dS (at 2 D) times its PK (at D), each summed over the splits first.
+// kFix (dQ): minus the row's sum of rounded dS (at 2 D) times its PK (at D), each summed over the splits first; the sum of dS before
+// rounding (at 2 D + 1) corrects the row's delta for the key side.
 template <bool kFp16, bool kFix>
 __global__ void __launch_bounds__(256) attn_bwd_sum_kernel(const float* parts, int splits, long long split_pitch, int pitch, int col0, int D, int H, int S,
-                                                           long long rows, void* out, long long sb, long long ss, long long sh) {
+                                                           long long rows, void* out, long long sb, long long ss, long long sh,
+                                                           const float* neg_delta, float* neg_delta_kv) {
   const int chunks = D / 8;
   const long long n = rows * chunks;
   for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < n; i += (long long)gridDim.x * 256) {
@@ -610,6 +626,12 @@ __global__ void __launch_bounds__(256) attn_bwd_sum_kernel(const float* parts, i
       float pk[8] = {}, r = 0.f;
       total(D + c, pk);
       for (int s = 0; s < splits; ++s) r += base[2 * D + s * split_pitch];
+      if (c == 0) {
+        float off = 0.f;
+        for (int s = 0; s < splits; ++s) off += base[2 * D + 1 + s * split_pitch];
+        const long long bh = row / S, si = bh * ((S + 127) / 128 * 128) + (row - bh * S);
+        neg_delta_kv[si] = neg_delta[si] - off;
+      }
 #pragma unroll
       for (int j = 0; j < 8; ++j) f[j] = fmaf(-r, pk[j], f[j]);
     }
@@ -679,7 +701,7 @@ Plan make_plan(const AttnBwdParams& p, bool gather) {
     w.heads_per_pass = (int)((bh + passes - 1) / passes);
     w.parts = up(w.heads_per_pass * head);
   }
-  w.total = 2 * w.stats + w.row_max + w.entries + w.starts + w.counts + w.parts;
+  w.total = 3 * w.stats + w.row_max + w.entries + w.starts + w.counts + w.parts;
   return w;
 }
 
@@ -709,16 +731,17 @@ int launch_dense(AttnBwdParams& p, const Plan& w, cudaStream_t stream) {
   dq<<<(unsigned)(items < sms ? items : sms), 384, kSmem, stream>>>(p, kv);
   if (p.splits > 1)
     attn_bwd_sum_kernel<kFp16, true><<<grid_of(bh * p.Sq * (p.D / 8)), 256, 0, stream>>>(
-        p.parts, p.splits, bh * p.Sq * (2 * p.D + 8), 2 * p.D + 8, 0, p.D, p.H, p.Sq, bh * p.Sq, p.dq, p.dq_stride[0], p.dq_stride[1], p.dq_stride[2]);
+        p.parts, p.splits, bh * p.Sq * (2 * p.D + 8), 2 * p.D + 8, 0, p.D, p.H, p.Sq, bh * p.Sq, p.dq, p.dq_stride[0], p.dq_stride[1], p.dq_stride[2],
+        p.neg_delta, p.neg_delta_kv);
   p.splits = w.kv_splits;
   items = bh * ((p.Sk + 127) / 128) * blocks * p.splits;
   dkv<<<(unsigned)(items < sms ? items : sms), 384, kSmem, stream>>>(p, qd);
   if (p.splits > 1) {
     const unsigned grid = grid_of(bh * p.Sk * (p.D / 8));
     attn_bwd_sum_kernel<kFp16, false><<<grid, 256, 0, stream>>>(p.parts, p.splits, bh * p.Sk * 2 * p.D, 2 * p.D, 0, p.D, p.H, p.Sk, bh * p.Sk, p.dk,
-                                                                p.dk_stride[0], p.dk_stride[1], p.dk_stride[2]);
+                                                                p.dk_stride[0], p.dk_stride[1], p.dk_stride[2], nullptr, nullptr);
     attn_bwd_sum_kernel<kFp16, false><<<grid, 256, 0, stream>>>(p.parts, p.splits, bh * p.Sk * 2 * p.D, 2 * p.D, p.D, p.D, p.H, p.Sk, bh * p.Sk, p.dv,
-                                                                p.dv_stride[0], p.dv_stride[1], p.dv_stride[2]);
+                                                                p.dv_stride[0], p.dv_stride[1], p.dv_stride[2], nullptr, nullptr);
   }
   return cudaGetLastError() == cudaSuccess ? 0 : -8;
 }
@@ -762,8 +785,9 @@ int launch_attn_bwd(AttnBwdParams& p, bool gather, bool fp16, void* workspace, c
   uint8_t* ws = static_cast<uint8_t*>(workspace);
   p.neg_lse2 = reinterpret_cast<float*>(ws);
   p.neg_delta = reinterpret_cast<float*>(ws + w.stats);
-  p.row_max = reinterpret_cast<unsigned int*>(ws + 2 * w.stats);
-  ws += 2 * w.stats + w.row_max;
+  p.neg_delta_kv = reinterpret_cast<float*>(ws + 2 * w.stats);
+  p.row_max = reinterpret_cast<unsigned int*>(ws + 3 * w.stats);
+  ws += 3 * w.stats + w.row_max;
   p.entry_row = reinterpret_cast<int32_t*>(ws);
   p.key_start = reinterpret_cast<int32_t*>(ws + w.entries);
   p.seg_count = reinterpret_cast<int32_t*>(ws + w.entries + w.starts);

@@ -384,7 +384,7 @@ __global__ void __launch_bounds__(kThreadsG, 1) attn_bwd_gather_dkv_kernel(const
       warp_copy_rows<DB>(s_base + (is_do ? L::kDO : L::kQ), 128, 0, 128, p.D,
                          reinterpret_cast<const uint8_t*>(src) + 2 * ((size_t)it.b * st[0] + (size_t)it.h * st[2]), 2 * (size_t)st[1], src,
                          [&](int r) { return row_of(it, r); });
-      cp_async16(s_base + L::kStat + (is_do ? 512 : 0) + lane * 16, (is_do ? p.neg_delta : p.neg_lse2) + ((size_t)it.bh * p.M + it.m) * 128 + lane * 4);
+      cp_async16(s_base + L::kStat + (is_do ? 512 : 0) + lane * 16, (is_do ? p.neg_delta_kv : p.neg_lse2) + ((size_t)it.bh * p.M + it.m) * 128 + lane * 4);
       cp_async_arrive_noinc(bar(L::kAFull));
     }
     cp_async_wait_all();

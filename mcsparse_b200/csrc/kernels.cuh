@@ -186,6 +186,7 @@ struct AttnBwdParams {
   float out_scale;                            // factor of dq and dk: the scale, or 0 where a single key leaves no gradient
   // workspace
   float *neg_lse2, *neg_delta;                // (B*H, M, 128): -(lse log2 e) (+ kBiasFp16), -rowsum(dout o out); -inf, 0 behind the last row
+  float* neg_delta_kv;                        // neg_delta less the row's sum of dS: what the key side uses (written with dQ)
   unsigned int* row_max;                      // fp16: (B*H, 2) largest norm of a row of dout, of v (as float bits)
   float* parts;                               // split launches: partial sums
   int splits;
