@@ -234,6 +234,12 @@ def lib() -> C.CDLL:
     return L
 
 
+def packed(cls, layout, *values):
+    """An argument structure from all of its values in order (`layout`: a ``struct.Struct`` of the same fields): one packing
+    operation where assigning a few dozen ctypes fields costs more than the launch."""
+    return cls.from_buffer_copy(layout.pack(*values))
+
+
 def launch(fn_name: str, args, device, where: str) -> None:
     """Call an entry point on the current torch stream of ``device``; raise on an argument error."""
     import torch

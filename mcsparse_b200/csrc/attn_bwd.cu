@@ -8,6 +8,8 @@
 // side's sums in tensor memory, takes P and dS straight out of tensor memory as the first operand of the next product, and
 // writes every result once.  The price is three products more (8 instead of 5): S and dP are computed on either side, and the
 // query side carries P K to correct dQ (below).
+#include <algorithm>
+
 #include "attn_bwd.cuh"
 
 namespace mcs {
@@ -19,8 +21,8 @@ using namespace bwd;
 constexpr int kMaxSmem = 232448;
 
 // ------------------------------------------------------------------------------------------------ row statistics
-// One CTA of 256 threads takes 16 rows at a time, 16 lanes each: neg_delta = -sum(dout * out) and neg_lse2 of every tile row
-// (memory-bound: dout and out are read once), and for fp16 the largest norms of rows of dout and of v.
+// Sixteen lanes per row, four rows at a time: neg_delta = -sum(dout * out) and neg_lse2 of every tile row (memory-bound: dout and out
+// are read once, eight 16-byte loads of a thread in flight), and for fp16 the largest norms of rows of dout and of v.
 template <bool kFp16>
 __device__ __forceinline__ float dot8(uint4 a, uint4 b, float acc) {
   const uint32_t x[4] = {a.x, a.y, a.z, a.w}, y[4] = {b.x, b.y, b.z, b.w};
@@ -38,72 +40,93 @@ __device__ __forceinline__ float dot8(uint4 a, uint4 b, float acc) {
 
 template <bool kFp16>
 __global__ void __launch_bounds__(256) attn_bwd_stats_kernel(const AttnBwdParams p) {
+  constexpr int kRows = 4;
   const int bh = blockIdx.y, h = bh % p.H, b = bh / p.H;
   const int l16 = threadIdx.x & 15, sub = threadIdx.x >> 4;
   const int rows = p.M * 128;
-  const int total = rows + (kFp16 ? p.Sk : 0);
   const int chunks = p.D / 8;
+  const uint8_t* gb = reinterpret_cast<const uint8_t*>(p.dout) + 2 * ((size_t)b * p.dout_stride[0] + (size_t)h * p.dout_stride[2]);
+  const uint8_t* ob = reinterpret_cast<const uint8_t*>(p.out) + 2 * ((size_t)b * p.out_stride[0] + (size_t)h * p.out_stride[2]);
   float m_do = 0.f, m_v = 0.f;
-  for (int base = blockIdx.x * 16; base < total; base += gridDim.x * 16) {
-    const int i = base + sub;
-    float dot = 0.f, sq = 0.f;
-    int row = -1;
-    if (i < rows) {
-      const int r = i & 127, pos = (i >> 7) * p.group_rows + r;
-      if (r < p.group_rows && pos < p.Sq) row = p.perm != nullptr ? (int)p.perm[(size_t)bh * p.Sq + pos] : pos;
-      if (row >= 0) {
-        const uint8_t* g = reinterpret_cast<const uint8_t*>(p.dout) + 2 * ((size_t)b * p.dout_stride[0] + (size_t)row * p.dout_stride[1] + (size_t)h * p.dout_stride[2]);
-        const uint8_t* o = reinterpret_cast<const uint8_t*>(p.out) + 2 * ((size_t)b * p.out_stride[0] + (size_t)row * p.out_stride[1] + (size_t)h * p.out_stride[2]);
-        for (int c = l16; c < chunks; c += 16) {
-          const uint4 x = *reinterpret_cast<const uint4*>(g + c * 16), y = *reinterpret_cast<const uint4*>(o + c * 16);
-          dot = dot8<kFp16>(x, y, dot);
-          if constexpr (kFp16) sq = dot8<kFp16>(x, x, sq);
+  for (int base = blockIdx.x * (16 * kRows); base < rows; base += gridDim.x * (16 * kRows)) {
+    int row[kRows];
+    float dot[kRows] = {}, sq[kRows] = {};
+#pragma unroll
+    for (int u = 0; u < kRows; ++u) {
+      const int i = base + u * 16 + sub, r = i & 127, pos = (i >> 7) * p.group_rows + r;
+      row[u] = -1;
+      if (i < rows && r < p.group_rows && pos < p.Sq) row[u] = p.perm != nullptr ? (int)p.perm[(size_t)bh * p.Sq + pos] : pos;
+    }
+    for (int c = l16; c < chunks; c += 16) {
+      uint4 x[kRows], y[kRows];
+#pragma unroll
+      for (int u = 0; u < kRows; ++u) {
+        x[u] = y[u] = make_uint4(0, 0, 0, 0);
+        if (row[u] >= 0) {
+          x[u] = *reinterpret_cast<const uint4*>(gb + 2 * (size_t)row[u] * p.dout_stride[1] + c * 16);
+          y[u] = *reinterpret_cast<const uint4*>(ob + 2 * (size_t)row[u] * p.out_stride[1] + c * 16);
         }
       }
-    } else if (i < total) {
-      const uint8_t* v = reinterpret_cast<const uint8_t*>(p.v) + 2 * ((size_t)b * p.v_stride[0] + (size_t)(i - rows) * p.v_stride[1] + (size_t)h * p.v_stride[2]);
-      for (int c = l16; c < chunks; c += 16) {
-        const uint4 x = *reinterpret_cast<const uint4*>(v + c * 16);
-        sq = dot8<kFp16>(x, x, sq);
+#pragma unroll
+      for (int u = 0; u < kRows; ++u) {
+        dot[u] = dot8<kFp16>(x[u], y[u], dot[u]);
+        if constexpr (kFp16) sq[u] = dot8<kFp16>(x[u], x[u], sq[u]);
       }
     }
 #pragma unroll
-    for (int off = 8; off >= 1; off >>= 1) {
-      dot += __shfl_xor_sync(0xffffffffu, dot, off);
-      if constexpr (kFp16) sq += __shfl_xor_sync(0xffffffffu, sq, off);
-    }
-    if (i < rows) {
-      if (l16 == 0) {
-        float nl = -INFINITY, nd = 0.f;                      // rows behind the last one: P = 0
-        if (row >= 0) {
-          const float l = p.lse[(size_t)bh * p.Sq + row];
+    for (int u = 0; u < kRows; ++u) {
+#pragma unroll
+      for (int off = 8; off >= 1; off >>= 1) {
+        dot[u] += __shfl_xor_sync(0xffffffffu, dot[u], off);
+        if constexpr (kFp16) sq[u] += __shfl_xor_sync(0xffffffffu, sq[u], off);
+      }
+      m_do = fmaxf(m_do, sq[u]);
+      const int i = base + u * 16 + sub;
+      if (l16 == 0 && i < rows) {
+        float nl = -INFINITY;                                // rows behind the last one: P = 0
+        if (row[u] >= 0) {
+          const float l = p.lse[(size_t)bh * p.Sq + row[u]];
           // (a row without keys has lse = -inf and no gradient)
           if (l != -INFINITY) nl = (kFp16 ? kBiasFp16 : 0.f) - l * 1.4426950408889634f;
-          nd = -dot;
         }
         p.neg_lse2[(size_t)bh * rows + i] = nl;
-        p.neg_delta[(size_t)bh * rows + i] = nd;
-        if (row < 0) p.neg_delta_kv[(size_t)bh * rows + i] = 0.f;      // (the others are written with dQ)
+        p.neg_delta[(size_t)bh * rows + i] = row[u] >= 0 ? -dot[u] : 0.f;
+        if (row[u] < 0) p.neg_delta_kv[(size_t)bh * rows + i] = 0.f;      // (the others are written with dQ)
       }
-      if constexpr (kFp16) m_do = fmaxf(m_do, sq);
-    } else if constexpr (kFp16) {
-      m_v = fmaxf(m_v, sq);
     }
   }
   if constexpr (kFp16) {
-    __shared__ float red[2][8];
+    const uint8_t* vb = reinterpret_cast<const uint8_t*>(p.v) + 2 * ((size_t)b * p.v_stride[0] + (size_t)h * p.v_stride[2]);
+    for (int base = blockIdx.x * (16 * kRows); base < p.Sk; base += gridDim.x * (16 * kRows)) {
+      float sq[kRows] = {};
+      for (int c = l16; c < chunks; c += 16) {
+        uint4 x[kRows];
+#pragma unroll
+        for (int u = 0; u < kRows; ++u) {
+          const int i = base + u * 16 + sub;
+          x[u] = i < p.Sk ? *reinterpret_cast<const uint4*>(vb + 2 * (size_t)i * p.v_stride[1] + c * 16) : make_uint4(0, 0, 0, 0);
+        }
+#pragma unroll
+        for (int u = 0; u < kRows; ++u) sq[u] = dot8<kFp16>(x[u], x[u], sq[u]);
+      }
+#pragma unroll
+      for (int u = 0; u < kRows; ++u) {
+#pragma unroll
+        for (int off = 8; off >= 1; off >>= 1) sq[u] += __shfl_xor_sync(0xffffffffu, sq[u], off);
+        m_v = fmaxf(m_v, sq[u]);
+      }
+    }
+    __shared__ float2 red[8];
 #pragma unroll
     for (int off = 16; off >= 1; off >>= 1) {
       m_do = fmaxf(m_do, __shfl_xor_sync(0xffffffffu, m_do, off));
       m_v = fmaxf(m_v, __shfl_xor_sync(0xffffffffu, m_v, off));
     }
-    if ((threadIdx.x & 31) == 0) { red[0][threadIdx.x >> 5] = m_do; red[1][threadIdx.x >> 5] = m_v; }
+    if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = make_float2(m_do, m_v);
     __syncthreads();
-    if (threadIdx.x < 2) {
-      float m = 0.f;
-      for (int i = 0; i < 8; ++i) m = fmaxf(m, red[threadIdx.x][i]);
-      // (non-negative floats compare as their bits; the largest of a set does not depend on the order)
-      atomicMax(p.row_max + 2 * bh + threadIdx.x, __float_as_uint(sqrtf(m) * 1.0001f));
+    if (threadIdx.x == 0) {
+      for (int i = 1; i < 8; ++i) { m_do = fmaxf(m_do, red[i].x); m_v = fmaxf(m_v, red[i].y); }
+      p.row_max[(size_t)bh * kMaxBlocks + blockIdx.x] = make_float2(sqrtf(m_do) * 1.0001f, sqrtf(m_v) * 1.0001f);
     }
   }
 }
@@ -115,9 +138,11 @@ __global__ void __launch_bounds__(256) attn_bwd_stats_kernel(const AttnBwdParams
 //   kDq, kDqGather   Q    dO   K    V      rows: queries                   PK += P K     dQ += dS K
 //   kDkv             K    V    Q    dO     rows: keys (S^T, dP^T)          dV += P^T dO  dK += dS^T Q
 // Scores lie with the resident row as the tensor-memory lane, so that P and dS are the first operands of the sums where they
-// are: P overwrites its scores and dS its dP.  Products of one thread execute in order, so S(t+1) may follow the sum that reads P(t)
-// without a wait, and dP(t+1) the one that reads dS(t).  Issue order: sum of P(t), S(t+1), sum of dS(t), dP(t+1); P of t+1 is computed
-// under the sum of dS(t) and dP(t+1), dS of t under the sum of P(t) and S(t+1).
+// are.  A softmax thread copies its scores to registers, which frees S for the next tile at once, and computes P there; when dP(t) is
+// complete it reads it and stores P and dS, 16 bits each, over it.  Issue order: sum of P(t), sum of dS(t), dP(t+1), S(t+2).  Products of
+// one thread execute in order, so dP(t+1) may follow the sums that read P(t) and dS(t) without a wait.  The exponentials of t+1 run
+// under the sum of dS(t) and dP(t+1); what the tensor pipe could wait for, dP(t) -> P stored, is covered by S(t+1).  (With P stored over
+// its scores, S(t+1) had to follow the sum of P(t), and the exponentials of t+1 that: @@OLD@@)
 //
 // PK: the rows of dS sum to zero, but those of its rounded form, with a delta from a rounded out, do not: they sum to r, and
 // dQ is off by r times the keys that a row looks at, which does not average out where these keys resemble one another (with
@@ -130,36 +155,44 @@ enum { kDq = 0, kDqGather = 1, kDkv = 2 };
 template <int DB, int TN>
 struct SmemB {
   using G = Geo<DB, TN>;
-  static constexpr int kRing = DB == 4 ? 3 : (DB == 2 ? 4 : 6);
+  static constexpr int kRing = DB == 4 ? 3 : (DB == 1 ? 8 : 5);
   static constexpr int kA0 = 0, kA1 = G::kResBytes;
   static constexpr int kRingOff = 2 * G::kResBytes;
   static constexpr int kStat = kRingOff + kRing * G::kTileBytes;           // kDkv: TN floats per slot, lse2 with Q, delta with dO; kDq: sums of dS
   static constexpr int kStatBytes = kRing * TN * 4 > 1536 ? kRing * TN * 4 : 1536;
   static constexpr int kBars = kStat + kStatBytes;
-  static constexpr int kFull = 0, kEmpty = kRing, kAFull = 2 * kRing, kAEmpty = kAFull + 1, kSFull = kAEmpty + 1, kDPFull = kSFull + 1,
+  static constexpr int kFull = 0, kEmpty = kRing, kAFull = 2 * kRing, kAEmpty = kAFull + 1, kSFull = kAEmpty + 1, kSFree = kSFull + 1, kDPFull = kSFree + 1,
                        kPReady = kDPFull + 1, kDSReady = kPReady + 1, kOFull = kDSReady + 1, kOFree = kOFull + 1, kRowSum = kOFree + 1,
                        kDrain = kRowSum + 1, kCount = kDrain + 1;
   static constexpr int kSlot = kBars + kCount * 8;
-  static constexpr int kDynamic = kSlot + 16 + 1024;
-  static constexpr uint32_t kColS = 0, kColDP = TN, kColA = 2 * TN, kWidth = DB == 4 ? 192 : DB * 64, kColB = kColA + kWidth;
+  static constexpr int kDynamic = kSlot + 16;
+  static constexpr uint32_t kColS = 0, kColDP = TN, kColA = 2 * TN, kWidth = DB > 2 ? 192 : DB * 64, kColB = kColA + kWidth;
 };
-static_assert(SmemB<2, 128>::kDynamic <= kMaxSmem && SmemB<4, 64>::kDynamic <= kMaxSmem && SmemB<1, 128>::kDynamic <= kMaxSmem, "must fit 227 KB");
-static_assert(SmemB<2, 128>::kColB + SmemB<2, 128>::kWidth <= 512 && SmemB<4, 64>::kColB + SmemB<4, 64>::kWidth <= 512, "tensor memory");
+template <int DB, int TN>
+constexpr bool fits = SmemB<DB, TN>::kDynamic <= kMaxSmem && SmemB<DB, TN>::kColB + SmemB<DB, TN>::kWidth <= 512;
+static_assert(fits<1, 128> && fits<2, 128> && fits<3, 64> && fits<4, 64>, "227 KB of shared memory, 512 columns of tensor memory");
 
-constexpr int kIssueWarp = 8, kLoadWarp0 = 9, kRingWarp0 = 11;   // issuer, two copies of resident tiles, then the ring's producers
+// Warps: eight softmax warps, the issuer, then for the dense modes the producers of the resident tiles and of the ring, for gathered keys
+// three warps that copy both (a thirteenth warp would leave 128 registers each instead of 168).
+constexpr int kIssueWarp = 8, kLoadWarp0 = 9, kThreadsB = 384;
 
 // Blocks of output columns: one, or two of 128 where tensor memory does not hold both sums at full width.
 __host__ __device__ constexpr int column_blocks(int D) { return D > 192 ? 2 : 1; }
 
 template <int DB, int TN, bool kFp16, int kMode>
-__global__ void __launch_bounds__(kMode == kDqGather ? 480 : 384, 1) attn_bwd_kernel(const AttnBwdParams p, const __grid_constant__ DenseTileMaps maps) {
+__global__ void __launch_bounds__(kThreadsB, 1) attn_bwd_kernel(const AttnBwdParams p, const __grid_constant__ DenseTileMaps maps,
+                                                                const __grid_constant__ DenseTileMaps res) {
   using L = SmemB<DB, TN>;
   using G = Geo<DB, TN>;
   constexpr bool kGather = kMode == kDqGather, kRowsAreKeys = kMode == kDkv;
   constexpr int R = L::kRing, HC = G::kHalf;
-  extern __shared__ __align__(1024) uint8_t smem_raw[];
-  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  // (no room for a manual alignment: the tiles need 1,024 bytes, which the declaration asks for and the host would be told if it failed)
+  extern __shared__ __align__(1024) uint8_t smem[];
   const uint32_t s_base = smem_u32(smem);
+  if (s_base & 1023u) {
+    if (threadIdx.x == 0) atomicCAS(p.status, 0, 1);
+    return;
+  }
   auto bar = [&](int i) { return s_base + L::kBars + 8u * i; };
   auto sRing = [&](int slot) { return s_base + L::kRingOff + slot * G::kTileBytes; };
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + L::kSlot);
@@ -205,10 +238,11 @@ __global__ void __launch_bounds__(kMode == kDqGather ? 480 : 384, 1) attn_bwd_ke
   };
 
   if (tid == 0) {
-    for (int i = 0; i < R; ++i) { mbar_init(bar(L::kFull + i), kGather ? 128 : 1); mbar_init(bar(L::kEmpty + i), 1); }
-    mbar_init(bar(L::kAFull), 64);
+    for (int i = 0; i < R; ++i) { mbar_init(bar(L::kFull + i), kGather ? TN : 1); mbar_init(bar(L::kEmpty + i), 1); }
+    mbar_init(bar(L::kAFull), kGather ? 256 : 1);
     mbar_init(bar(L::kAEmpty), 1);
     mbar_init(bar(L::kSFull), 1);
+    mbar_init(bar(L::kSFree), kSoftmaxWarps);
     mbar_init(bar(L::kDPFull), 1);
     mbar_init(bar(L::kPReady), kSoftmaxWarps);
     mbar_init(bar(L::kDSReady), kSoftmaxWarps);
@@ -234,7 +268,7 @@ __global__ void __launch_bounds__(kMode == kDqGather ? 480 : 384, 1) attn_bwd_ke
     };
     const int x = warp >> 2, r_in = (warp & 3) * 32 + lane;
     const uint32_t lane_addr = (static_cast<uint32_t>(warp & 3) * 32u) << 16;
-    // each half of the columns keeps its packed operands inside its own columns: no thread overwrites what another still reads
+    // each half of the columns keeps its 16-bit operands inside its own columns of dP: no thread overwrites what another still reads
     const uint32_t tS = tmem + L::kColS + x * HC + lane_addr, tDP = tmem + L::kColDP + x * HC + lane_addr;
     const unsigned long long scale2 = f2_pack(p.scale_log2, p.scale_log2);
     int g = 0, ic = 0;
@@ -242,7 +276,7 @@ __global__ void __launch_bounds__(kMode == kDqGather ? 480 : 384, 1) attn_bwd_ke
 #pragma unroll 1
     for (int item = blockIdx.x; item < n_items && ok; item += gridDim.x) {
       const Item it = decode(item);
-      const float c = ds_scale<kFp16>(p.row_max, it.bh);
+      const float c = ds_scale<kFp16>(p, it.bh);
       const unsigned long long c2 = f2_pack(c, c);
       unsigned long long nl2 = 0, nd2 = 0, rs[2] = {0, 0}, es[2] = {0, 0};   // kDq: this row's statistics, sums of its dS rounded and not
       if constexpr (!kRowsAreKeys) {
@@ -264,6 +298,8 @@ __global__ void __launch_bounds__(kMode == kDqGather ? 480 : 384, 1) attn_bwd_ke
 #pragma unroll
         for (int q = 0; q < HC / 32; ++q) tmem_ld32(tS + q * 32, *reinterpret_cast<uint32_t(*)[32]>(&sc[q * 32]));
         tmem_wait_ld();
+        tc_fence_before();
+        warp_arrive(bar(L::kSFree));
 #pragma unroll
         for (int i = 0; i < HC; i += 4) {
           unsigned long long l0 = nl2, l1 = nl2;
@@ -278,9 +314,6 @@ __global__ void __launch_bounds__(kMode == kDqGather ? 480 : 384, 1) attn_bwd_ke
           sc[i + 1] = __float_as_uint(ex2_approx(y0.y));
           sc[i + 2] = __float_as_uint(ex2_approx(y1.x));
           sc[i + 3] = __float_as_uint(ex2_approx(y1.y));
-          if constexpr (kMode != kDq) {
-            if (i % 16 == 12) store_packed<kFp16>(tS + (i - 12) / 2, &sc[i - 12]);
-          }
         }
         if constexpr (kMode == kDq) {
           // key positions behind the sequence end (zero rows of the last tile): exp2(-lse2) could be anything
@@ -290,53 +323,57 @@ __global__ void __launch_bounds__(kMode == kDqGather ? 480 : 384, 1) attn_bwd_ke
             for (int i = 0; i < HC; ++i)
               if (i >= rem) sc[i] = 0;
           }
-#pragma unroll
-          for (int q = 0; q < HC / 16; ++q) store_packed<kFp16>(tS + q * 8, &sc[q * 16]);
         }
-        tmem_wait_st();
-        tc_fence_before();
-        warp_arrive(bar(L::kPReady));
         ok = mbar_wait(bar(L::kDPFull), g & 1, p.status, 132);
         if constexpr (kRowsAreKeys) ok = ok && mbar_wait(bar(L::kFull + n1 % R), (n1 / R) & 1, p.status, 133);
         if (!ok) break;
         tc_fence_after();
-        constexpr int kStep = kMode == kDq ? HC : 32;        // (more would spill: 136 registers with 480 threads, 168 with 384)
+        // dP in steps of 32 columns, all in flight at once where the registers allow it; P goes over the first half of this thread's
+        // columns as soon as those are read, dS over the second half
+        constexpr int kSteps = HC / 32;
+        constexpr bool kAll = false;
+        uint32_t dp[kAll ? HC : 32], pk[HC / 2];
+        tmem_ld32(tDP, *reinterpret_cast<uint32_t(*)[32]>(&dp[0]));
+        if constexpr (kAll && kSteps == 2) tmem_ld32(tDP + 32, *reinterpret_cast<uint32_t(*)[32]>(&dp[kAll && kSteps == 2 ? 32 : 0]));
+        tmem_wait_ld();
 #pragma unroll
-        for (int s0 = 0; s0 < HC; s0 += kStep) {
-          uint32_t dp[kStep];
+        for (int q = 0; q < HC / 16; ++q) store_packed<kFp16>(tDP + q * 8, &sc[q * 16]);
+        tmem_wait_st();
+        tc_fence_before();
+        warp_arrive(bar(L::kPReady));
 #pragma unroll
-          for (int q = 0; q < kStep / 32; ++q) tmem_ld32(tDP + s0 + q * 32, *reinterpret_cast<uint32_t(*)[32]>(&dp[q * 32]));
-          tmem_wait_ld();
+        for (int st = 0; st < kSteps; ++st) {
+          if (!kAll && st > 0) {
+            tmem_ld32(tDP + 32, *reinterpret_cast<uint32_t(*)[32]>(&dp[0]));
+            tmem_wait_ld();
+          }
 #pragma unroll
-          for (int q = 0; q < kStep / 16; ++q) {
-            uint32_t pk[8];
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-              const int e = q * 16 + 4 * i;
-              unsigned long long e0 = nd2, e1 = nd2;
-              if constexpr (kRowsAreKeys) {
-                const ulonglong2 l = dlt[(s0 + e) / 4];
-                e0 = l.x;
-                e1 = l.y;
-              }
-              unsigned long long d0 = f2_add(f2_pack(__uint_as_float(dp[e]), __uint_as_float(dp[e + 1])), e0);
-              unsigned long long d1 = f2_add(f2_pack(__uint_as_float(dp[e + 2]), __uint_as_float(dp[e + 3])), e1);
-              if constexpr (kFp16) { d0 = f2_mul(d0, c2); d1 = f2_mul(d1, c2); }
-              d0 = f2_mul(f2_pack(__uint_as_float(sc[s0 + e]), __uint_as_float(sc[s0 + e + 1])), d0);
-              d1 = f2_mul(f2_pack(__uint_as_float(sc[s0 + e + 2]), __uint_as_float(sc[s0 + e + 3])), d1);
-              const float2 y0 = f2_unpack(d0), y1 = f2_unpack(d1);
-              pk[2 * i] = pack16<kFp16>(y0.x, y0.y);
-              pk[2 * i + 1] = pack16<kFp16>(y1.x, y1.y);
-              if constexpr (!kRowsAreKeys) {
-                es[0] = f2_add(es[0], d0);
-                es[1] = f2_add(es[1], d1);
-                rs[0] = f2_add(rs[0], unpack16<kFp16>(pk[2 * i]));
-                rs[1] = f2_add(rs[1], unpack16<kFp16>(pk[2 * i + 1]));
-              }
+          for (int i = 0; i < 8; ++i) {
+            const int e = st * 32 + 4 * i, d = kAll ? e : 4 * i;
+            unsigned long long e0 = nd2, e1 = nd2;
+            if constexpr (kRowsAreKeys) {
+              const ulonglong2 l = dlt[e / 4];
+              e0 = l.x;
+              e1 = l.y;
             }
-            tmem_st8(tDP + (s0 + q * 16) / 2, pk);
+            unsigned long long d0 = f2_add(f2_pack(__uint_as_float(dp[d]), __uint_as_float(dp[d + 1])), e0);
+            unsigned long long d1 = f2_add(f2_pack(__uint_as_float(dp[d + 2]), __uint_as_float(dp[d + 3])), e1);
+            if constexpr (kFp16) { d0 = f2_mul(d0, c2); d1 = f2_mul(d1, c2); }
+            d0 = f2_mul(f2_pack(__uint_as_float(sc[e]), __uint_as_float(sc[e + 1])), d0);
+            d1 = f2_mul(f2_pack(__uint_as_float(sc[e + 2]), __uint_as_float(sc[e + 3])), d1);
+            const float2 y0 = f2_unpack(d0), y1 = f2_unpack(d1);
+            pk[e / 2] = pack16<kFp16>(y0.x, y0.y);
+            pk[e / 2 + 1] = pack16<kFp16>(y1.x, y1.y);
+            if constexpr (!kRowsAreKeys) {
+              es[0] = f2_add(es[0], d0);
+              es[1] = f2_add(es[1], d1);
+              rs[0] = f2_add(rs[0], unpack16<kFp16>(pk[e / 2]));
+              rs[1] = f2_add(rs[1], unpack16<kFp16>(pk[e / 2 + 1]));
+            }
           }
         }
+#pragma unroll
+        for (int q = 0; q < HC / 16; ++q) tmem_st8(tDP + HC / 2 + q * 8, *reinterpret_cast<const uint32_t(*)[8]>(&pk[q * 8]));
         tmem_wait_st();
         tc_fence_before();
         warp_arrive(bar(L::kDSReady));
@@ -372,6 +409,8 @@ __global__ void __launch_bounds__(kMode == kDqGather ? 480 : 384, 1) attn_bwd_ke
       const int64_t* st = kRowsAreKeys ? (second ? p.dk_stride : p.dv_stride) : p.dq_stride;
       void* dst = kRowsAreKeys ? (second ? p.dk : p.dv) : p.dq;
       uint8_t* optr = reinterpret_cast<uint8_t*>(dst) + 2 * ((size_t)it.b * st[0] + safe * st[1] + (size_t)it.h * st[2]);
+      // (32-byte stores where every row starts on a 32-byte boundary)
+      const bool wide = ((reinterpret_cast<uintptr_t>(dst) | (uintptr_t)(2 * (st[0] | st[1] | st[2]))) & 31) == 0;
       const int S = kRowsAreKeys ? p.Sk : p.Sq;
       // a row of partial sums: dK | dV, or dQ | PK | the sums of dS (padded to 8 floats)
       const int pitch = kRowsAreKeys ? 2 * p.D : 2 * p.D + 8;
@@ -397,23 +436,23 @@ __global__ void __launch_bounds__(kMode == kDqGather ? 480 : 384, 1) attn_bwd_ke
             f[i] = fmaf(-fix * unbias, __uint_as_float(ra[i]), __uint_as_float(rb[i])) * w;
           }
         }
+        const int col = it.c0 + cc;
+        if (row >= 0 && p.splits > 1) {
 #pragma unroll
-        for (int q = 0; q < 2; ++q) {
-          const int col = it.c0 + cc + q * 8;
-          if (row < 0 || col >= p.D) break;
-          if (p.splits > 1) {
-            float4* o = reinterpret_cast<float4*>(part + (kRowsAreKeys && x == 0 ? p.D : 0) + col);
-            o[0] = make_float4(f[q * 8], f[q * 8 + 1], f[q * 8 + 2], f[q * 8 + 3]);
-            o[1] = make_float4(f[q * 8 + 4], f[q * 8 + 5], f[q * 8 + 6], f[q * 8 + 7]);
-            if constexpr (!kRowsAreKeys) {
-              o = reinterpret_cast<float4*>(part + p.D + col);
-              o[0] = make_float4(e[q * 8], e[q * 8 + 1], e[q * 8 + 2], e[q * 8 + 3]);
-              o[1] = make_float4(e[q * 8 + 4], e[q * 8 + 5], e[q * 8 + 6], e[q * 8 + 7]);
-            }
+          for (int q = 0; q < 16; q += 8) {
+            if (col + q >= p.D) break;
+            store8(part + (kRowsAreKeys && x == 0 ? p.D : 0) + col + q, f + q);
+            if constexpr (!kRowsAreKeys) store8(part + p.D + col + q, e + q);
+          }
+        } else if (row >= 0) {
+          float o[8];
+#pragma unroll
+          for (int i = 0; i < 8; ++i) o[i] = __uint_as_float(pack16<kFp16>(f[2 * i], f[2 * i + 1]));
+          if (wide && col + 16 <= p.D) {
+            store8(reinterpret_cast<float*>(optr + 2 * col), o);
           } else {
-            *reinterpret_cast<uint4*>(optr + 2 * col) =
-                make_uint4(pack16<kFp16>(f[q * 8], f[q * 8 + 1]), pack16<kFp16>(f[q * 8 + 2], f[q * 8 + 3]),
-                           pack16<kFp16>(f[q * 8 + 4], f[q * 8 + 5]), pack16<kFp16>(f[q * 8 + 6], f[q * 8 + 7]));
+            *reinterpret_cast<float4*>(optr + 2 * col) = make_float4(o[0], o[1], o[2], o[3]);
+            if (col + 16 <= p.D) *reinterpret_cast<float4*>(optr + 2 * col + 16) = make_float4(o[4], o[5], o[6], o[7]);
           }
         }
         __syncwarp();
@@ -450,11 +489,31 @@ __global__ void __launch_bounds__(kMode == kDqGather ? 480 : 384, 1) attn_bwd_ke
         if (leader && j < kd) mma_f16_ss(d, desc_lo(alo + (j >> 2) * (16384 >> 4) + in), desc_lo(blo + (j >> 2) * (TN * 128 >> 4) + in), idesc_s, j > 0);
       }
     };
+    // sum over a tile of T rows: the operand of half x of the rows lies HC columns behind that of the first half
     auto sum = [&](uint32_t d, uint32_t a, int load, const Item& it, uint32_t idesc, bool first) {
       const uint32_t blo = lo_mnmajor(sRing(load % R) + (it.c0 >> 6) * TN * 128, TN * 128);
 #pragma unroll
       for (int j = 0; j < TN / 16; ++j)
         if (leader) mma_f16_ts(d, a + (j / (TN / 32)) * HC + (j % (TN / 32)) * 8, desc_lo(blo + j * (2048 >> 4)), idesc, !first || j > 0);
+    };
+    // S of the tile with running number gs: its scores' columns are free once the tile before has been copied out
+    auto score_tile = [&](int gs) {
+      wait_full(2 * gs);
+      if (ok && gs > 0) ok = mbar_wait(bar(L::kSFree), (gs - 1) & 1, p.status, 143);
+      if (!ok) return;
+      tc_fence_after();
+      scores(tmem + L::kColS, s_base + L::kA0, 2 * gs);
+      if (leader) tc_commit(bar(L::kSFull));
+    };
+    auto dp_tile = [&](int gs, bool last) {
+      wait_full(2 * gs + 1);
+      if (!ok) return;
+      scores(tmem + L::kColDP, s_base + L::kA1, 2 * gs + 1);
+      if (leader) {
+        tc_commit(bar(L::kDPFull));
+        if (!kRowsAreKeys) tc_commit(bar(L::kEmpty + (2 * gs + 1) % R));
+        if (last) tc_commit(bar(L::kAEmpty));
+      }
     };
 #pragma unroll 1
     for (int item = blockIdx.x; item < n_items && ok; item += gridDim.x) {
@@ -462,20 +521,12 @@ __global__ void __launch_bounds__(kMode == kDqGather ? 480 : 384, 1) attn_bwd_ke
       const uint32_t idesc_o = mma_idesc(kFmt, kFmt, 0, 1, 128, it.ncol);
       ok = mbar_wait(bar(L::kAFull), ic & 1, p.status, 137);
       if (!ok) break;
-      fence_proxy_async_smem();
+      if constexpr (kGather) fence_proxy_async_smem();
       tc_fence_after();
-      wait_full(2 * g);
+      score_tile(g);
+      if (ok) dp_tile(g, it.t1 - it.t0 == 1);
+      if (ok && it.t1 - it.t0 > 1) score_tile(g + 1);
       if (!ok) break;
-      scores(tmem + L::kColS, s_base + L::kA0, 2 * g);
-      if (leader) tc_commit(bar(L::kSFull));
-      wait_full(2 * g + 1);
-      if (!ok) break;
-      scores(tmem + L::kColDP, s_base + L::kA1, 2 * g + 1);
-      if (leader) {
-        tc_commit(bar(L::kDPFull));
-        if (!kRowsAreKeys) tc_commit(bar(L::kEmpty + (2 * g + 1) % R));
-        if (it.t1 - it.t0 == 1) tc_commit(bar(L::kAEmpty));
-      }
 #pragma unroll 1
       for (int t = it.t0; t < it.t1; ++t, ++g) {
         const bool first = t == it.t0, last = t == it.t1 - 1;
@@ -484,32 +535,19 @@ __global__ void __launch_bounds__(kMode == kDqGather ? 480 : 384, 1) attn_bwd_ke
         if (ok && first && ic > 0) ok = mbar_wait(bar(L::kOFree), (ic - 1) & 1, p.status, 139);
         if (!ok) break;
         tc_fence_after();
-        sum(tmem + L::kColA, tmem + L::kColS, kRowsAreKeys ? n + 1 : n, it, idesc_o, first);
+        sum(tmem + L::kColA, tmem + L::kColDP, kRowsAreKeys ? n + 1 : n, it, idesc_o, first);
         if (kRowsAreKeys && leader) tc_commit(bar(L::kEmpty + (n + 1) % R));
-        if (!last) {
-          wait_full(n + 2);
-          if (!ok) break;
-          scores(tmem + L::kColS, s_base + L::kA0, n + 2);
-          if (leader) tc_commit(bar(L::kSFull));
-        }
         ok = mbar_wait(bar(L::kDSReady), g & 1, p.status, 140);
         if (!ok) break;
         tc_fence_after();
-        sum(tmem + L::kColB, tmem + L::kColDP, n, it, idesc_o, first);
+        sum(tmem + L::kColB, tmem + L::kColDP + HC / 2, n, it, idesc_o, first);
         if (leader) {
           tc_commit(bar(L::kEmpty + n % R));
           if (last) tc_commit(bar(L::kOFull));
         }
-        if (!last) {
-          wait_full(n + 3);
-          if (!ok) break;
-          scores(tmem + L::kColDP, s_base + L::kA1, n + 3);
-          if (leader) {
-            tc_commit(bar(L::kDPFull));
-            if (!kRowsAreKeys) tc_commit(bar(L::kEmpty + (n + 3) % R));
-            if (t + 2 == it.t1) tc_commit(bar(L::kAEmpty));
-          }
-        }
+        if (!last) dp_tile(g + 1, t + 2 == it.t1);
+        if (ok && t + 2 < it.t1) score_tile(g + 2);
+        if (!ok) break;
       }
       ++ic;
     }
@@ -520,28 +558,95 @@ __global__ void __launch_bounds__(kMode == kDqGather ? 480 : 384, 1) attn_bwd_ke
     }
     __syncwarp();
     tc_fence_before();
-  } else if (warp < kRingWarp0) {
-    // ---- the resident tiles of an item: A0 by the first warp, A1 by the second (queries through the permutation)
-    const bool is_a1 = warp != kLoadWarp0;
-    const void* src = kRowsAreKeys ? (is_a1 ? p.v : p.k) : (is_a1 ? p.dout : p.q);
-    const int64_t* st = kRowsAreKeys ? (is_a1 ? p.v_stride : p.k_stride) : (is_a1 ? p.dout_stride : p.q_stride);
-    int ic = 0;
+  } else if (kGather) {
+    // ---- gathered keys: the warps take batches of 32 rows in turn.  The resident tiles of an item follow its first pair of T tiles,
+    // which do not have to wait for the item before to be done with A0 and A1.
+    constexpr int kBatches = TN / 32, kWarps = 3;
+    const int w = warp - kLoadWarp0;
+    int n = 0, ic = 0, batch = 0;
     bool ok = true;
+    // indices of the tile that is copied, and of the next one of the item, in flight meanwhile
+    int key[kBatches], next[kBatches];
+    auto fetch = [&](const int32_t* gi, int t, int (&dst)[kBatches]) {
+#pragma unroll
+      for (int q = 0; q < kBatches; ++q) dst[q] = __ldg(gi + (size_t)t * TN + q * 32 + lane);
+    };
 #pragma unroll 1
-    for (int item = blockIdx.x; item < n_items && ok; item += gridDim.x) {
+    for (int item = blockIdx.x; item < n_items && ok; item += gridDim.x, ++ic) {
       const Item it = decode(item);
-      if (ic > 0) ok = mbar_wait(bar(L::kAEmpty), (ic - 1) & 1, p.status, 141);
-      if (!ok) break;
-      warp_copy_rows<DB>(s_base + (is_a1 ? L::kA1 : L::kA0), 128, 0, 128, p.D,
-                         reinterpret_cast<const uint8_t*>(src) + 2 * ((size_t)it.b * st[0] + (size_t)it.h * st[2]), 2 * (size_t)st[1], src,
-                         [&](int r) { return row_of(it, r); });
-      cp_async_arrive_noinc(bar(L::kAFull));
-      ++ic;
+      const int32_t* gi = p.gi + ((size_t)it.bh * p.M + it.m) * p.gather_len;
+      const uint8_t* kb = reinterpret_cast<const uint8_t*>(p.k) + 2 * ((size_t)it.b * p.k_stride[0] + (size_t)it.h * p.k_stride[2]);
+      const uint8_t* vb = reinterpret_cast<const uint8_t*>(p.v) + 2 * ((size_t)it.b * p.v_stride[0] + (size_t)it.h * p.v_stride[2]);
+      fetch(gi, it.t0, key);
+#pragma unroll 1
+      for (int t = it.t0; t < it.t1 && ok; ++t) {
+        if (t + 1 < it.t1) fetch(gi, t + 1, next);
+#pragma unroll 1
+        for (int is_t1 = 0; is_t1 < 2; ++is_t1, ++n) {
+          const int slot = n % R;
+          if (n >= R) ok = mbar_wait(bar(L::kEmpty + slot), (n / R - 1) & 1, p.status, 142);
+          if (!ok) break;
+#pragma unroll
+          for (int q = 0; q < kBatches; ++q) {
+            if (batch == w) {
+              warp_copy_rows<DB>(sRing(slot), TN, q * 32, min(max(key[q], 0), p.Sk - 1), p.D, is_t1 ? vb : kb,
+                                 2 * (size_t)(is_t1 ? p.v_stride[1] : p.k_stride[1]), p.k);
+              cp_async_arrive_noinc(bar(L::kFull + slot));
+            }
+            batch = batch == kWarps - 1 ? 0 : batch + 1;
+          }
+        }
+        if (!ok) break;
+        if (t == it.t0) {
+          if (ic > 0) ok = mbar_wait(bar(L::kAEmpty), (ic - 1) & 1, p.status, 141);
+          if (!ok) break;
+#pragma unroll 1
+          for (int q = 0; q < 8; ++q) {
+            if (batch == w) {
+              const bool a1 = q >= 4;
+              const int64_t* ast = a1 ? p.dout_stride : p.q_stride;
+              const uint8_t* src = reinterpret_cast<const uint8_t*>(a1 ? p.dout : p.q) + 2 * ((size_t)it.b * ast[0] + (size_t)it.h * ast[2]);
+              warp_copy_rows<DB>(s_base + (a1 ? L::kA1 : L::kA0), 128, (q & 3) * 32, row_of(it, (q & 3) * 32 + lane), p.D, src, 2 * (size_t)ast[1], p.q);
+              cp_async_arrive_noinc(bar(L::kAFull));
+            }
+            batch = batch == kWarps - 1 ? 0 : batch + 1;
+          }
+        }
+#pragma unroll
+        for (int q = 0; q < kBatches; ++q) key[q] = next[q];
+      }
     }
     cp_async_wait_all();
     tc_fence_before();
-  } else {
-    // ---- the ring: T0(0), T1(0), T0(1), ...
+  } else if (warp == kLoadWarp0) {
+    // ---- the resident tiles of an item, by TMA
+    const bool leader = elect_one();
+    int ic = 0;
+    bool ok = true;
+#pragma unroll 1
+    for (int item = blockIdx.x; item < n_items && ok; item += gridDim.x, ++ic) {
+      const Item it = decode(item);
+      if (ic > 0) ok = mbar_wait(bar(L::kAEmpty), (ic - 1) & 1, p.status, 141);
+      if (!ok) break;
+      if (leader) {
+        mbar_arrive_expect_tx(bar(L::kAFull), 2 * G::kResBytes);
+#pragma unroll
+        for (int half = 0; half < 128 / TN; ++half) {
+          int c0[4] = {0, 0, 0, 0}, c1[4] = {0, 0, 0, 0};
+          c0[res.k_pos_h] = it.h; c0[res.k_pos_b] = it.b; c0[res.k_pos_row] = it.m * 128 + half * TN;
+          c1[res.v_pos_h] = it.h; c1[res.v_pos_b] = it.b; c1[res.v_pos_row] = it.m * 128 + half * TN;
+#pragma unroll
+          for (int cb = 0; cb < DB; ++cb) {
+            tma_load_4d(s_base + L::kA0 + cb * 16384 + half * TN * 128, res.k, cb * 64, c0[1], c0[2], c0[3], bar(L::kAFull));
+            tma_load_4d(s_base + L::kA1 + cb * 16384 + half * TN * 128, res.v, cb * 64, c1[1], c1[2], c1[3], bar(L::kAFull));
+          }
+        }
+      }
+    }
+    if (!ok && ic > 0) mbar_wait_quiet(bar(L::kAFull), (ic - 1) & 1, 1 << 16);   // copies in flight
+    tc_fence_before();
+  } else if (warp == kLoadWarp0 + 1) {
+    // ---- the ring: T0(0), T1(0), T0(1), ... by TMA
     const bool leader = elect_one();
     int n = 0;
     bool ok = true;
@@ -549,27 +654,15 @@ __global__ void __launch_bounds__(kMode == kDqGather ? 480 : 384, 1) attn_bwd_ke
     for (int item = blockIdx.x; item < n_items && ok; item += gridDim.x) {
       const Item it = decode(item);
       int c0[4] = {0, 0, 0, 0}, c1[4] = {0, 0, 0, 0};
-      if constexpr (!kGather) {
-        c0[maps.k_pos_h] = it.h; c0[maps.k_pos_b] = it.b;
-        c1[maps.v_pos_h] = it.h; c1[maps.v_pos_b] = it.b;
-      }
+      c0[maps.k_pos_h] = it.h; c0[maps.k_pos_b] = it.b;
+      c1[maps.v_pos_h] = it.h; c1[maps.v_pos_b] = it.b;
 #pragma unroll 1
       for (int e = 2 * it.t0; e < 2 * it.t1 && ok; ++e, ++n) {
         const bool is_t1 = e & 1;
         const int slot = n % R;
         if (n >= R) ok = mbar_wait(bar(L::kEmpty + slot), (n / R - 1) & 1, p.status, 142);
         if (!ok) break;
-        if constexpr (kGather) {
-          constexpr int kRows = TN / 4;
-          const int w = warp - kRingWarp0;
-          const int32_t* gi = p.gi + ((size_t)it.bh * p.M + it.m) * p.gather_len + (size_t)(e >> 1) * TN;
-          const int64_t* st = is_t1 ? p.v_stride : p.k_stride;
-          const void* src = is_t1 ? p.v : p.k;
-          warp_copy_rows<DB>(sRing(slot), TN, w * kRows, kRows, p.D,
-                             reinterpret_cast<const uint8_t*>(src) + 2 * ((size_t)it.b * st[0] + (size_t)it.h * st[2]), 2 * (size_t)st[1], src,
-                             [&](int r) { return min(max(gi[r], 0), p.Sk - 1); });
-          cp_async_arrive_noinc(bar(L::kFull + slot));
-        } else if (leader) {
+        if (leader) {
           mbar_arrive_expect_tx(bar(L::kFull + slot), G::kTileBytes + (kRowsAreKeys ? TN * 4 : 0));
           const void* map = is_t1 ? static_cast<const void*>(maps.v) : static_cast<const void*>(maps.k);
           int co[4] = {0, is_t1 ? c1[1] : c0[1], is_t1 ? c1[2] : c0[2], is_t1 ? c1[3] : c0[3]};
@@ -583,11 +676,8 @@ __global__ void __launch_bounds__(kMode == kDqGather ? 480 : 384, 1) attn_bwd_ke
         }
       }
     }
-    if constexpr (kGather) {
-      cp_async_wait_all();
-    } else if (!ok) {
+    if (!ok)
       for (int i = n > R ? n - R : 0; i < n; ++i) mbar_wait_quiet(bar(L::kFull + i % R), (i / R) & 1, 1 << 16);   // copies in flight
-    }
     tc_fence_before();
   }
 
@@ -665,24 +755,24 @@ int pick_splits(long long items, int T, int sms) {
 // passes would only add launches with a partly filled last wave.
 constexpr size_t kPartsBytes = 4ull << 30;
 
-struct Plan { int dq_splits, kv_splits, segs, heads_per_pass; size_t stats, row_max, entries, starts, counts, parts, total; };
+struct Plan { int dq_splits, kv_splits, segs, heads_per_pass; size_t stats, row_max, entries, starts, counts, blocks, parts, total; };
 
 constexpr size_t kAlign = 256;
 size_t up(size_t n) { return (n + kAlign - 1) / kAlign * kAlign; }
 
-int padded_blocks(int D) { return D <= 64 ? 1 : (D <= 128 ? 2 : 4); }
+int padded_blocks(int D) { return D <= 64 ? 1 : (D <= 128 ? 2 : (D <= 192 ? 3 : 4)); }
 
 Plan make_plan(const AttnBwdParams& p, bool gather) {
   // (the split rule uses the B200's 148 SMs, not the current device's: sizes must not depend on the device that asks)
   constexpr int kSms = 148;
   Plan w{};
-  const int TN = padded_blocks(p.D) == 4 ? 64 : 128;
+  const int TN = padded_blocks(p.D) > 2 ? 64 : 128;
   const long long bh = (long long)p.B * p.H;
   const int blocks = column_blocks(p.D);
   w.dq_splits = gather ? 1 : pick_splits(bh * p.M * blocks, (p.Sk + TN - 1) / TN, kSms);
   w.kv_splits = gather ? 1 : pick_splits(bh * ((p.Sk + 127) / 128) * blocks, (p.Sq + TN - 1) / TN, kSms);
   w.stats = up((size_t)bh * p.M * 128 * 4);
-  w.row_max = up((size_t)bh * 8);
+  w.row_max = up((size_t)bh * kMaxBlocks * 8);
   size_t a = w.dq_splits > 1 ? (size_t)w.dq_splits * bh * p.Sq * (2 * p.D + 8) * 4 : 0, b = w.kv_splits > 1 ? (size_t)w.kv_splits * bh * p.Sk * 2 * p.D * 4 : 0;
   w.parts = up(a > b ? a : b);
   if (gather) {
@@ -693,6 +783,7 @@ Plan make_plan(const AttnBwdParams& p, bool gather) {
     w.entries = up((size_t)bh * p.M * p.gather_len * 4);
     w.starts = up((size_t)bh * (p.Sk + 1) * 4);
     w.counts = up((size_t)bh * w.segs * p.Sk * 4);
+    w.blocks = up((size_t)bh * ((p.Sk + 1023) / 1024) * 4);
     // the contributions of as many heads at a time as fit kPartsBytes, at least one
     const size_t head = (size_t)p.M * p.gather_len * 2 * p.D * 4;
     const long long fit = (long long)(kPartsBytes / head);
@@ -701,7 +792,7 @@ Plan make_plan(const AttnBwdParams& p, bool gather) {
     w.heads_per_pass = (int)((bh + passes - 1) / passes);
     w.parts = up(w.heads_per_pass * head);
   }
-  w.total = 3 * w.stats + w.row_max + w.entries + w.starts + w.counts + w.parts;
+  w.total = 3 * w.stats + w.row_max + w.entries + w.starts + w.counts + w.blocks + w.parts;
   return w;
 }
 
@@ -728,14 +819,14 @@ int launch_dense(AttnBwdParams& p, const Plan& w, cudaStream_t stream) {
   auto grid_of = [](long long n) { return (unsigned)(n / 256 + 1 < 148 * 8 ? n / 256 + 1 : 148 * 8); };
   p.splits = w.dq_splits;
   long long items = bh * p.M * blocks * p.splits;
-  dq<<<(unsigned)(items < sms ? items : sms), 384, kSmem, stream>>>(p, kv);
+  dq<<<(unsigned)(items < sms ? items : sms), kThreadsB, kSmem, stream>>>(p, kv, qd);
   if (p.splits > 1)
     attn_bwd_sum_kernel<kFp16, true><<<grid_of(bh * p.Sq * (p.D / 8)), 256, 0, stream>>>(
         p.parts, p.splits, bh * p.Sq * (2 * p.D + 8), 2 * p.D + 8, 0, p.D, p.H, p.Sq, bh * p.Sq, p.dq, p.dq_stride[0], p.dq_stride[1], p.dq_stride[2],
         p.neg_delta, p.neg_delta_kv);
   p.splits = w.kv_splits;
   items = bh * ((p.Sk + 127) / 128) * blocks * p.splits;
-  dkv<<<(unsigned)(items < sms ? items : sms), 384, kSmem, stream>>>(p, qd);
+  dkv<<<(unsigned)(items < sms ? items : sms), kThreadsB, kSmem, stream>>>(p, qd, kv);
   if (p.splits > 1) {
     const unsigned grid = grid_of(bh * p.Sk * (p.D / 8));
     attn_bwd_sum_kernel<kFp16, false><<<grid, 256, 0, stream>>>(p.parts, p.splits, bh * p.Sk * 2 * p.D, 2 * p.D, 0, p.D, p.H, p.Sk, bh * p.Sk, p.dk,
@@ -754,24 +845,28 @@ int launch_gather_dq(AttnBwdParams& p, cudaStream_t stream) {
   const int sms = sm_count();
   p.splits = 1;
   const long long items = (long long)p.B * p.H * p.M * column_blocks(p.D);
-  dq<<<(unsigned)(items < sms ? items : sms), 480, kSmem, stream>>>(p, DenseTileMaps{});
+  dq<<<(unsigned)(items < sms ? items : sms), kThreadsB, kSmem, stream>>>(p, DenseTileMaps{}, DenseTileMaps{});
   return cudaGetLastError() == cudaSuccess ? 0 : -8;
 }
 
 template <bool kFp16>
 int launch_type(AttnBwdParams& p, const Plan& w, bool gather, cudaStream_t stream) {
-  if (kFp16 && cudaMemsetAsync(p.row_max, 0, (size_t)p.B * p.H * 8, stream) != cudaSuccess) return -8;
-  const int rows = p.M * 128 + (kFp16 ? p.Sk : 0);
-  const int per = (rows + 15) / 16;
-  attn_bwd_stats_kernel<kFp16><<<dim3((unsigned)(per < 256 ? per : 256), (unsigned)(p.B * p.H)), 256, 0, stream>>>(p);
+  // (fp16: at most kMaxBlocks CTAs per head, whose maxima are kept apart)
+  const int bh = p.B * p.H, per = (std::max(p.M * 128, kFp16 ? p.Sk : 0) + 63) / 64;
+  p.max_blocks = std::min(per, kFp16 ? kMaxBlocks : std::max(1, 148 * 8 * 4 / bh));
+  attn_bwd_stats_kernel<kFp16><<<dim3((unsigned)p.max_blocks, (unsigned)bh), 256, 0, stream>>>(p);
   if (gather) {
     const int db = padded_blocks(p.D);
-    const int rc = db == 1 ? launch_gather_dq<1, 128, kFp16>(p, stream) : (db == 2 ? launch_gather_dq<2, 128, kFp16>(p, stream) : launch_gather_dq<4, 64, kFp16>(p, stream));
+    const int rc = db == 1   ? launch_gather_dq<1, 128, kFp16>(p, stream)
+                   : db == 2 ? launch_gather_dq<2, 128, kFp16>(p, stream)
+                   : db == 3 ? launch_gather_dq<3, 64, kFp16>(p, stream)
+                             : launch_gather_dq<4, 64, kFp16>(p, stream);
     return rc != 0 ? rc : launch_attn_bwd_gather_dkv(p, kFp16, w.segs, w.heads_per_pass, stream);
   }
   switch (padded_blocks(p.D)) {
     case 1: return launch_dense<1, 128, kFp16>(p, w, stream);
     case 2: return launch_dense<2, 128, kFp16>(p, w, stream);
+    case 3: return launch_dense<3, 64, kFp16>(p, w, stream);
     default: return launch_dense<4, 64, kFp16>(p, w, stream);
   }
 }
@@ -786,12 +881,13 @@ int launch_attn_bwd(AttnBwdParams& p, bool gather, bool fp16, void* workspace, c
   p.neg_lse2 = reinterpret_cast<float*>(ws);
   p.neg_delta = reinterpret_cast<float*>(ws + w.stats);
   p.neg_delta_kv = reinterpret_cast<float*>(ws + 2 * w.stats);
-  p.row_max = reinterpret_cast<unsigned int*>(ws + 3 * w.stats);
+  p.row_max = reinterpret_cast<float2*>(ws + 3 * w.stats);
   ws += 3 * w.stats + w.row_max;
   p.entry_row = reinterpret_cast<int32_t*>(ws);
   p.key_start = reinterpret_cast<int32_t*>(ws + w.entries);
   p.seg_count = reinterpret_cast<int32_t*>(ws + w.entries + w.starts);
-  p.parts = reinterpret_cast<float*>(ws + w.entries + w.starts + w.counts);
+  p.block_sum = reinterpret_cast<int32_t*>(ws + w.entries + w.starts + w.counts);
+  p.parts = reinterpret_cast<float*>(ws + w.entries + w.starts + w.counts + w.blocks);
   return fp16 ? launch_type<true>(p, w, gather, stream) : launch_type<false>(p, w, gather, stream);
 }
 

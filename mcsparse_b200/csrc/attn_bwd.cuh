@@ -23,11 +23,20 @@ namespace bwd {
 constexpr float kBiasFp16 = 14.f;
 constexpr int kSoftmaxWarps = 8;       // warps 0-3 take the first half of a score tile's columns, 4-7 the second; lane == row
 
-// Power of two by which dS / 2^14 may be multiplied (see above), from the largest row norms; 1 for bf16.
+// Power of two by which dS / 2^14 may be multiplied (see above), from the largest row norms; 1 for bf16.  A whole warp calls it.
+constexpr int kMaxBlocks = 32;          // CTAs per head of the statistics, each of which leaves its own maxima
 template <bool kFp16>
-__device__ __forceinline__ float ds_scale(const unsigned int* row_max, int bh) {
+__device__ __forceinline__ float ds_scale(const AttnBwdParams& p, int bh) {
   if constexpr (!kFp16) return 1.f;
-  const float m = 2.f * __uint_as_float(row_max[2 * bh]) * __uint_as_float(row_max[2 * bh + 1]);
+  const int lane = threadIdx.x & 31;
+  const float2* parts = p.row_max + (size_t)bh * kMaxBlocks;
+  float2 v = lane < p.max_blocks ? parts[lane] : make_float2(0.f, 0.f);
+#pragma unroll
+  for (int off = 16; off >= 1; off >>= 1) {
+    v.x = fmaxf(v.x, __shfl_xor_sync(0xffffffffu, v.x, off));
+    v.y = fmaxf(v.y, __shfl_xor_sync(0xffffffffu, v.y, off));
+  }
+  const float m = 2.f * v.x * v.y;
   if (!(m > 0.f) || isinf(m)) return 1.f;
   int e;
   frexpf(m, &e);                        // m < 2^e
@@ -50,24 +59,35 @@ __device__ __forceinline__ uint32_t lo_kmajor(uint32_t saddr) { return ((saddr &
 // MN-major operand: `block_bytes` from one block of 64 columns to the next
 __device__ __forceinline__ uint32_t lo_mnmajor(uint32_t saddr, uint32_t block_bytes) { return ((saddr & 0x3FFFFu) >> 4) | ((block_bytes >> 4) << 16); }
 
-// One warp copies `rows` rows (row_of(i): source row, or -1 for zeros) of D elements into a tile of column blocks of
-// block_rows rows, from tile row r0 on.  Columns from D on are zeros.
-template <int DB, typename RowOf>
-__device__ __forceinline__ void warp_copy_rows(uint32_t tile, int block_rows, int r0, int rows, int D, const uint8_t* base, size_t row_bytes,
-                                               const void* any, RowOf row_of) {
+// One warp copies 32 rows (lane i's row from source row `mine`, or zeros if that is negative) of D elements into rows r0 .. r0 + 31 of a
+// tile of column blocks of block_rows rows.  Columns from D on are zeros.
+template <int DB>
+__device__ __forceinline__ void warp_copy_rows(uint32_t tile, int block_rows, int r0, int mine, int D, const uint8_t* base, size_t row_bytes, const void* any) {
   const int lane = threadIdx.x & 31;
-  constexpr int kChunks = DB * 8;
-  for (int rb = 0; rb < rows; rb += 32) {
-    const int mine = rb + lane < rows ? row_of(r0 + rb + lane) : -1;
-    const int n = min(32, rows - rb) * kChunks;
-#pragma unroll 4
-    for (int e = lane; e < n; e += 32) {
-      const int rl = e / kChunks, c = e % kChunks;
+  constexpr int kChunks = DB * 8;                            // 16-byte chunks of a row
+  if constexpr (32 % kChunks == 0) {
+    // a lane keeps its chunk, 32 / kChunks rows at a time
+    constexpr int kRows = 32 / kChunks;
+    const int c = lane % kChunks, sub = lane / kChunks;
+    const uint8_t* src = base + c * 16;
+    const uint32_t dst = tile + (c >> 3) * (block_rows * 128);
+    const bool in = c * 8 < D;
+#pragma unroll 8
+    for (int i = 0; i < kChunks; ++i) {
+      const int rl = i * kRows + sub, r = r0 + rl;
       const int id = __shfl_sync(0xffffffffu, mine, rl);
-      const int r = r0 + rb + rl;
-      const uint32_t dst = tile + (c >> 3) * (block_rows * 128) + r * 128 + (((c & 7) ^ (r & 7)) << 4);
-      if (id >= 0 && c * 8 < D) cp_async16(dst, base + (size_t)id * row_bytes + c * 16);
-      else cp_async16_zfill(dst, any, 0);
+      const uint32_t at = dst + r * 128 + (((c & 7) ^ (r & 7)) << 4);
+      if (in && id >= 0) cp_async16(at, src + (size_t)(uint32_t)id * row_bytes);
+      else cp_async16_zfill(at, any, 0);
+    }
+  } else {
+#pragma unroll 4
+    for (int i = 0; i < kChunks; ++i) {
+      const int e = i * 32 + lane, rl = e / kChunks, c = e % kChunks, r = r0 + rl;
+      const int id = __shfl_sync(0xffffffffu, mine, rl);
+      const uint32_t at = tile + (c >> 3) * (block_rows * 128) + r * 128 + (((c & 7) ^ (r & 7)) << 4);
+      if (id >= 0 && c * 8 < D) cp_async16(at, base + (size_t)(uint32_t)id * row_bytes + c * 16);
+      else cp_async16_zfill(at, any, 0);
     }
   }
 }
@@ -95,6 +115,13 @@ __device__ __forceinline__ void store_packed(uint32_t taddr, const uint32_t* v) 
 #pragma unroll
   for (int i = 0; i < 8; ++i) pk[i] = pack16<kFp16>(__uint_as_float(v[2 * i]), __uint_as_float(v[2 * i + 1]));
   tmem_st8(taddr, pk);
+}
+
+// eight fp32 values as one 32-byte store: a row's thread fills whole sectors
+__device__ __forceinline__ void store8(float* dst, const float* f) {
+  asm volatile("st.global.v8.f32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(dst), "f"(f[0]), "f"(f[1]), "f"(f[2]), "f"(f[3]), "f"(f[4]), "f"(f[5]),
+               "f"(f[6]), "f"(f[7])
+               : "memory");
 }
 
 }  // namespace bwd

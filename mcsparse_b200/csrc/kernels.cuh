@@ -167,7 +167,7 @@ struct RotaryParams {
   unsigned char axis[kRotaryMaxPairs];
   int B, L, D, n_pairs, pos64, inverse;
   float magnitude;
-  int units, rot_units, heads_per_chunk, head_chunks;   // set by the launch
+  int units, rot_units, unit_threads, tokens_per_cta, heads_per_cta;   // set by the launch
 };
 int launch_rotary(RotaryParams& p, int type, bool half, cudaStream_t stream);
 
@@ -187,12 +187,13 @@ struct AttnBwdParams {
   // workspace
   float *neg_lse2, *neg_delta;                // (B*H, M, 128): -(lse log2 e) (+ kBiasFp16), -rowsum(dout o out); -inf, 0 behind the last row
   float* neg_delta_kv;                        // neg_delta less the row's sum of dS: what the key side uses (written with dQ)
-  unsigned int* row_max;                      // fp16: (B*H, 2) largest norm of a row of dout, of v (as float bits)
+  float2* row_max;                            // fp16: (B*H, 32) largest norms of rows of dout and of v that each CTA of the statistics saw
+  int max_blocks;                             // CTAs per head of the statistics (at most 32)
   float* parts;                               // split launches: partial sums
   int splits;
   // gather: entries that name key j of head bh lie at rows [key_start[bh][j], key_start[bh][j + 1]) of that head's block of partial
   // sums, in the order of groups; entry_row[bh][m][slot] is the row of an entry
-  int32_t *entry_row, *key_start, *seg_count;
+  int32_t *entry_row, *key_start, *seg_count, *block_sum;
   int bh0, bh_count;                          // heads of this launch
 };
 int64_t attn_bwd_workspace_bytes(const AttnBwdParams& p, bool gather, bool fp16);

@@ -48,118 +48,129 @@ struct alignas(N * sizeof(T)) Pack { T v[N]; };
 // kVec: elements per access; the host picks 16 bytes, or single elements where a stride, an address or the size of the rotated
 // part does not allow 16 bytes.  kHalf: pairs (p, p + n) instead of (2p, 2p + 1).
 template <int kType, bool kHalf, int kVec>
-__global__ void __launch_bounds__(kThreadsR) rotary_kernel(const __grid_constant__ RotaryParams p) {
+struct Layout {
   using E = Elem<kType>;
   using T = typename E::T;
-  // pairs per unit, and the elements of either member that one unit reads
-  constexpr int kPairs = kHalf ? kVec : (kVec > 1 ? kVec / 2 : 1);
-  constexpr bool kSplit = kHalf || kVec == 1;                // the members of a pair come from two accesses
   using V = Pack<T, kVec>;
-  const long long idx = (long long)blockIdx.x * kThreadsR + threadIdx.x;
-  const int unit = (int)(idx % p.units);
-  const long long rest = idx / p.units;
-  const long long tokens = (long long)p.B * p.L;
-  const long long chunk = rest / tokens;
-  if (chunk >= p.head_chunks) return;
-  const long long token = rest - chunk * tokens;
-  const long long b = token / p.L, row = token - b * p.L;
-  const bool rotates = unit < p.rot_units;
+  static constexpr int kPairs = kHalf ? kVec : (kVec > 1 ? kVec / 2 : 1);   // pairs of one unit
+  static constexpr bool kSplit = kHalf || kVec == 1;                        // the members of a pair come from two accesses
+};
 
-  float c[kPairs], s[kPairs];
-  int ea, eb;                                                // first elements of the two accesses
-  if (rotates) {
-    const long long base = b * p.p_stride[0] + row * p.p_stride[1];
+// `heads` rows of one token, `stride` elements apart: rotated by (c, s), or copied
+template <int kType, bool kHalf, int kVec, bool kRotate>
+__device__ __forceinline__ void walk_heads(const typename Elem<kType>::T* x, typename Elem<kType>::T* y, long long xs, long long ys, int heads, int n_pairs,
+                                           const float* c, const float* s) {
+  using Y = Layout<kType, kHalf, kVec>;
+  using E = typename Y::E;
+  using V = typename Y::V;
+  const int second = kHalf ? n_pairs : 1;                    // where the other member of a pair is
+  auto turn = [&](V& a, V& b) {
+    if constexpr (!kRotate) return;
+    if constexpr (Y::kSplit) {
 #pragma unroll
-    for (int j = 0; j < kPairs; ++j) {
-      const int pr = unit * kPairs + j;
-      const long long at = base + (long long)p.axis[pr] * p.p_stride[2];
-      const long long pos = p.pos64 ? reinterpret_cast<const long long*>(p.positions)[at]
-                                    : (long long)reinterpret_cast<const int*>(p.positions)[at];
-      const unsigned long long turn = (unsigned long long)pos * p.turns[pr];
-      // the upper 32 bits as a signed fraction of half a turn: [-1, 1), relative rounding 2^-25
-      const float half_turns = (float)(int)(turn >> 32) * 4.656612873077393e-10f;
-      sincospif(half_turns, &s[j], &c[j]);
-      c[j] *= p.magnitude;
-      s[j] *= p.inverse ? -p.magnitude : p.magnitude;
+      for (int j = 0; j < Y::kPairs; ++j) {
+        const float f = E::get(a.v[j]), g = E::get(b.v[j]);
+        a.v[j] = E::put(fmaf(f, c[j], -g * s[j]));
+        b.v[j] = E::put(fmaf(f, s[j], g * c[j]));
+      }
+    } else {
+#pragma unroll
+      for (int j = 0; j < Y::kPairs; ++j) {
+        const float f = E::get(a.v[2 * j]), g = E::get(a.v[2 * j + 1]);
+        a.v[2 * j] = E::put(fmaf(f, c[j], -g * s[j]));
+        a.v[2 * j + 1] = E::put(fmaf(f, s[j], g * c[j]));
+      }
     }
-    ea = kHalf ? unit * kVec : unit * (kVec > 1 ? kVec : 2);
-    eb = kHalf ? ea + p.n_pairs : ea + 1;
-  } else {
-    ea = eb = 2 * p.n_pairs + (unit - p.rot_units) * kVec;
+  };
+  constexpr bool kTwo = Y::kSplit && kRotate;
+  constexpr int kUnroll = kTwo ? 4 : 8;                      // loads in flight: eight of up to 16 bytes per thread
+  int h = 0;
+  for (; h + kUnroll <= heads; h += kUnroll, x += kUnroll * xs, y += kUnroll * ys) {
+    V a[kUnroll], b[kUnroll];
+#pragma unroll
+    for (int u = 0; u < kUnroll; ++u) {
+      a[u] = *reinterpret_cast<const V*>(x + u * xs);
+      if constexpr (kTwo) b[u] = *reinterpret_cast<const V*>(x + u * xs + second);
+    }
+#pragma unroll
+    for (int u = 0; u < kUnroll; ++u) {
+      turn(a[u], b[u]);
+      *reinterpret_cast<V*>(y + u * ys) = a[u];
+      if constexpr (kTwo) *reinterpret_cast<V*>(y + u * ys + second) = b[u];
+    }
   }
+  for (; h < heads; ++h, x += xs, y += ys) {
+    V a, b;
+    a = *reinterpret_cast<const V*>(x);
+    if constexpr (kTwo) b = *reinterpret_cast<const V*>(x + second);
+    turn(a, b);
+    *reinterpret_cast<V*>(y) = a;
+    if constexpr (kTwo) *reinterpret_cast<V*>(y + second) = b;
+  }
+}
 
-  const int heads = p.H[0] + p.H[1];
-  const int h_begin = (int)chunk * p.heads_per_chunk;
-  const int h_end = min(heads, h_begin + p.heads_per_chunk);
-  constexpr int kUnroll = kSplit ? 2 : 4;
-  for (int h0 = h_begin; h0 < h_end; h0 += kUnroll) {
-    V xa[kUnroll], xb[kUnroll];
+// A CTA takes `tokens_per_cta` tokens with `unit_threads` threads each; blockIdx.y is a run of heads of q and k together.
+template <int kType, bool kHalf, int kVec>
+__global__ void __launch_bounds__(kThreadsR) rotary_kernel(const __grid_constant__ RotaryParams p) {
+  using Y = Layout<kType, kHalf, kVec>;
+  using T = typename Y::T;
+  constexpr int kPairs = Y::kPairs;
+  const int sub = threadIdx.x / p.unit_threads, lane = threadIdx.x - sub * p.unit_threads;
+  const long long token = (long long)blockIdx.x * p.tokens_per_cta + sub;
+  if (sub >= p.tokens_per_cta || token >= (long long)p.B * p.L) return;
+  const int b = (int)(token / p.L), row = (int)(token - (long long)b * p.L);
+  const int h0 = blockIdx.y * p.heads_per_cta, h1 = min(h0 + p.heads_per_cta, p.H[0] + p.H[1]);
+  for (int unit = lane; unit < p.units; unit += p.unit_threads) {
+    const bool rotates = unit < p.rot_units;
+    float c[kPairs], s[kPairs];
+    if (rotates) {
+      const long long base = b * p.p_stride[0] + row * p.p_stride[1];
 #pragma unroll
-    for (int u = 0; u < kUnroll; ++u) {
-      const int h = h0 + u;
-      if (h < h_end) {
-        const int t = h >= p.H[0];
-        const T* x = reinterpret_cast<const T*>(p.x[t]) + b * p.x_stride[t][0] + row * p.x_stride[t][1] +
-                     (long long)(h - (t ? p.H[0] : 0)) * p.x_stride[t][2];
-        xa[u] = *reinterpret_cast<const V*>(x + ea);
-        if (kSplit && rotates) xb[u] = *reinterpret_cast<const V*>(x + eb);
+      for (int j = 0; j < kPairs; ++j) {
+        const int pr = unit * kPairs + j;
+        const long long at = base + (long long)p.axis[pr] * p.p_stride[2];
+        const long long pos = p.pos64 ? reinterpret_cast<const long long*>(p.positions)[at]
+                                      : (long long)reinterpret_cast<const int*>(p.positions)[at];
+        const unsigned long long turn = (unsigned long long)pos * p.turns[pr];
+        // the upper 32 bits as a signed fraction of half a turn: [-1, 1), relative rounding 2^-25
+        const float half_turns = (float)(int)(turn >> 32) * 4.656612873077393e-10f;
+        sincospif(half_turns, &s[j], &c[j]);
+        c[j] *= p.magnitude;
+        s[j] *= p.inverse ? -p.magnitude : p.magnitude;
       }
     }
+    const int e = rotates ? (kHalf ? unit * kVec : unit * (kVec > 1 ? kVec : 2)) : 2 * p.n_pairs + (unit - p.rot_units) * kVec;
 #pragma unroll
-    for (int u = 0; u < kUnroll; ++u) {
-      const int h = h0 + u;
-      if (h >= h_end) break;
-      const int t = h >= p.H[0];
-      T* y = reinterpret_cast<T*>(p.y[t]) + b * p.y_stride[t][0] + row * p.y_stride[t][1] +
-             (long long)(h - (t ? p.H[0] : 0)) * p.y_stride[t][2];
-      if (rotates) {
-        if constexpr (kSplit) {
-          V ya, yb;
-#pragma unroll
-          for (int j = 0; j < kPairs; ++j) {
-            const float a = E::get(xa[u].v[j]), d = E::get(xb[u].v[j]);
-            ya.v[j] = E::put(fmaf(a, c[j], -d * s[j]));
-            yb.v[j] = E::put(fmaf(a, s[j], d * c[j]));
-          }
-          *reinterpret_cast<V*>(y + ea) = ya;
-          *reinterpret_cast<V*>(y + eb) = yb;
-        } else {
-          V ya;
-#pragma unroll
-          for (int j = 0; j < kPairs; ++j) {
-            const float a = E::get(xa[u].v[2 * j]), d = E::get(xa[u].v[2 * j + 1]);
-            ya.v[2 * j] = E::put(fmaf(a, c[j], -d * s[j]));
-            ya.v[2 * j + 1] = E::put(fmaf(a, s[j], d * c[j]));
-          }
-          *reinterpret_cast<V*>(y + ea) = ya;
-        }
-      } else {
-        *reinterpret_cast<V*>(y + ea) = xa[u];
-      }
+    for (int t = 0; t < 2; ++t) {
+      // this CTA's heads of tensor t
+      const int first = t == 0 ? h0 : max(h0 - p.H[0], 0), end = t == 0 ? min(h1, p.H[0]) : h1 - p.H[0];
+      if (first >= end) continue;
+      const T* x = reinterpret_cast<const T*>(p.x[t]) + b * p.x_stride[t][0] + row * p.x_stride[t][1] + first * p.x_stride[t][2] + e;
+      T* y = reinterpret_cast<T*>(p.y[t]) + b * p.y_stride[t][0] + row * p.y_stride[t][1] + first * p.y_stride[t][2] + e;
+      if (rotates) walk_heads<kType, kHalf, kVec, true>(x, y, p.x_stride[t][2], p.y_stride[t][2], end - first, p.n_pairs, c, s);
+      else walk_heads<kType, kHalf, kVec, false>(x, y, p.x_stride[t][2], p.y_stride[t][2], end - first, p.n_pairs, c, s);
     }
   }
 }
 
 template <int kType, bool kHalf, int kVec>
 int launch_variant(RotaryParams& p, bool copy_rest, cudaStream_t stream) {
-  constexpr int kPairs = kHalf ? kVec : (kVec > 1 ? kVec / 2 : 1);
-  p.rot_units = p.n_pairs / kPairs;
+  p.rot_units = p.n_pairs / Layout<kType, kHalf, kVec>::kPairs;
   p.units = p.rot_units + (copy_rest ? (p.D - 2 * p.n_pairs) / kVec : 0);
   if (p.units == 0) return 0;
+  p.unit_threads = p.units < kThreadsR ? p.units : kThreadsR;
+  p.tokens_per_cta = kThreadsR / p.unit_threads;
   const int heads = p.H[0] + p.H[1];
-  const long long per_head = (long long)p.B * p.L * p.units;
-  // Few tokens: a thread takes fewer heads, so that the launch still fills the GPU (148 SMs x 8 CTAs); many tokens: up to
-  // kMaxHeads heads share one computation of the angles.
+  const long long tokens = (long long)p.B * p.L, ctas = (tokens + p.tokens_per_cta - 1) / p.tokens_per_cta;
+  if (ctas > 0x7fffffffLL) return -10;
+  // Up to kMaxHeads heads share one computation of the angles; with few tokens a CTA takes fewer, so that the launch still
+  // fills the GPU (148 SMs x 8 CTAs).
   constexpr int kMaxHeads = 16;
-  const long long want = 148LL * 8 * kThreadsR;
-  long long per = per_head >= want ? kMaxHeads : per_head * heads / want;
-  if (per < 1) per = 1;
-  if (per > kMaxHeads) per = kMaxHeads;
-  p.heads_per_chunk = (int)per;
-  p.head_chunks = (heads + p.heads_per_chunk - 1) / p.heads_per_chunk;
-  const long long blocks = (per_head * p.head_chunks + kThreadsR - 1) / kThreadsR;
-  if (blocks > 0x7fffffffLL) return -10;
-  rotary_kernel<kType, kHalf, kVec><<<(unsigned)blocks, kThreadsR, 0, stream>>>(p);
+  long long per = ctas * heads / (148 * 8);
+  per = per < 1 ? 1 : (per > kMaxHeads ? kMaxHeads : per);
+  if ((heads + per - 1) / per > 65535) per = (heads + 65534) / 65535;
+  p.heads_per_cta = (int)per;
+  rotary_kernel<kType, kHalf, kVec><<<dim3((unsigned)ctas, (unsigned)((heads + per - 1) / per)), kThreadsR, 0, stream>>>(p);
   return cudaGetLastError() == cudaSuccess ? 0 : -8;
 }
 

@@ -508,9 +508,9 @@ def flash_attn_gather_kv_backward_func(
     if isinstance(gather_kv_indices, PackedIndices):
         with torch.cuda.device(q.device):
             gather_kv_indices = gather_kv_indices.unpack()
-    dq, dk, dv = (torch.empty_like(t) if t.stride(-1) == 1 else torch.empty(t.shape, dtype=t.dtype, device=t.device) for t in (q, k, v))
-    dov, qv, kv, vv, ov = (attn_bwd.readable(t.detach()) for t in (dout, q, k, v, out))
-    attn_bwd.launch_backward("mcs_gather_attn_bwd", dov, qv, kv, vv, ov, lse.detach().contiguous(), dq, dk, dv, softmax_scale,
+    dq, dk, dv = (attn_bwd.gradient_like(t) for t in (q, k, v))
+    dov, qv, kv, vv, ov = (attn_bwd.readable(t) for t in (dout, q, k, v, out))
+    attn_bwd.launch_backward("mcs_gather_attn_bwd", dov, qv, kv, vv, ov, lse.contiguous(), dq, dk, dv, softmax_scale,
                              gather_kv_indices, gather_kv_lengths, perm, group_rows)
     return dq, dk, dv
 

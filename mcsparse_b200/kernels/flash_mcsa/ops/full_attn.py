@@ -104,10 +104,9 @@ def full_attention_backward(dout: Tensor, q: Tensor, k: Tensor, v: Tensor, out: 
         raise RuntimeError("dense attention runs on a CUDA device only; there is no CPU path")
     if k.device != q.device or v.device != q.device:
         raise ValueError("q, k and v must be on one device")
-    dq, dk, dv = (torch.empty_like(t) if t.stride(-1) == 1 else torch.empty(t.shape, dtype=t.dtype, device=t.device) for t in (q, k, v))
-    dov, qv, kv, vv, ov = (attn_bwd.readable(t.detach().transpose(1, 2)) for t in (dout, q, k, v, out))
-    attn_bwd.launch_backward("mcs_dense_attn_bwd", dov, qv, kv, vv, ov, lse.detach().contiguous(), dq.transpose(1, 2), dk.transpose(1, 2),
-                             dv.transpose(1, 2), scale)
+    dq, dk, dv = (attn_bwd.gradient_like(t) for t in (q, k, v))
+    dov, qv, kv, vv, ov = (attn_bwd.readable(t) for t in (dout, q, k, v, out))
+    attn_bwd.launch_backward("mcs_dense_attn_bwd", dov, qv, kv, vv, ov, lse.contiguous(), dq, dk, dv, scale, heads_first=True)
     return dq, dk, dv
 
 

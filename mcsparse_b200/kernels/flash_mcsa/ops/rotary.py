@@ -12,6 +12,7 @@ from __future__ import annotations
 
 import ctypes as C
 import math
+import struct
 from decimal import Decimal, localcontext
 from typing import Optional, Sequence, Tuple, Union
 
@@ -21,6 +22,8 @@ from torch import Tensor
 from mcsparse_b200 import _lib
 
 _DTYPES = {torch.bfloat16: _lib.MCS_DTYPE_BF16, torch.float16: _lib.MCS_DTYPE_FP16, torch.float32: _lib.MCS_DTYPE_FP32}
+_ARGS = struct.Struct("4Q12qQ3q2Q11if")     # the fields of mcs_rotary_args
+assert _ARGS.size == C.sizeof(_lib.RotaryArgs)
 _TWO_PI = 2 * Decimal("3.14159265358979323846264338327950288419716939937510582")
 
 
@@ -107,64 +110,75 @@ class RotaryEmbedding:
         self._axis = (C.c_uint8 * len(axis))(*axis)
 
     # ------------------------------------------------------------------------------------------ launches
-    def _check(self, tensors: Sequence[Tensor], positions: Tensor) -> Tensor:
-        """The positions as a (B or 1, L, axes) view; raises on arguments that the kernel does not take."""
+    def _check(self, tensors: Sequence[Tensor], positions: Tensor) -> Tuple[int, int, int]:
+        """The positions' (batch, row, axis) strides; raises on arguments that the kernel does not take."""
         if not 1 <= len(tensors) <= 2:
             raise ValueError(f"one or two tensors are rotated at a time, got {len(tensors)}")
         x = tensors[0]
+        dtype, device = x.dtype, x.device
         for t in tensors:
-            if t.dim() != 4 or t.shape[3] != self.head_dim:
-                raise ValueError(f"expected (B, L, H, {self.head_dim}) tensors, got {tuple(t.shape)}")
-            if t.shape[:2] != x.shape[:2]:
-                raise ValueError(f"batch and length must agree, got {tuple(x.shape)} and {tuple(t.shape)}")
-            if t.dtype not in _DTYPES or t.dtype != x.dtype:
+            shape = t.shape
+            if len(shape) != 4 or shape[3] != self.head_dim:
+                raise ValueError(f"expected (B, L, H, {self.head_dim}) tensors, got {tuple(shape)}")
+            if shape[:2] != x.shape[:2]:
+                raise ValueError(f"batch and length must agree, got {tuple(x.shape)} and {tuple(shape)}")
+            if t.dtype not in _DTYPES or t.dtype != dtype:
                 raise TypeError(f"rotary positions need bf16, fp16 or fp32 tensors of one dtype, got {t.dtype}")
         B, L = x.shape[:2]
         axes = len(self.axis_pairs)
         if positions.dtype not in (torch.int32, torch.int64):
             raise TypeError(f"positions must be int32 or int64, got {positions.dtype}")
-        p = positions.unsqueeze(-1) if axes == 1 else positions
-        if p.dim() == 2:
-            p = p.unsqueeze(0)
-        if p.dim() != 3 or p.shape[0] not in (1, B) or p.shape[1:] != (L, axes):
+        shape, strides = tuple(positions.shape), positions.stride()
+        if axes == 1:
+            shape, strides = shape + (1,), strides + (0,)
+        if len(shape) == 2:
+            shape, strides = (1,) + shape, (0,) + strides
+        if len(shape) != 3 or shape[0] not in (1, B) or shape[1] != L or shape[2] != axes:
             lead = f"({L},) or ({B}, {L})" if axes == 1 else f"({L}, {axes}) or ({B}, {L}, {axes})"
             raise ValueError(f"positions must have shape {lead}, got {tuple(positions.shape)}")
-        if not all(t.is_cuda for t in tensors):
-            raise RuntimeError("rotary positions run on a CUDA device only; there is no CPU path")
-        if any(t.device != x.device for t in (*tensors, positions)):
+        for t in tensors:
+            if not t.is_cuda:
+                raise RuntimeError("rotary positions run on a CUDA device only; there is no CPU path")
+            if t.device != device:
+                raise ValueError("tensors and positions must be on one device")
+        if positions.device != device:
             raise ValueError("tensors and positions must be on one device")
-        return p.expand(B, L, axes)
+        return strides if shape[0] == B else (0, strides[1], strides[2])
 
     def _launch(self, tensors: Sequence[Tensor], positions: Tensor, inverse: bool, inplace: bool) -> Tuple[Tensor, ...]:
-        p = self._check(tensors, positions)
+        p_stride = self._check(tensors, positions)
         if inplace:
             for t in tensors:
                 if t.stride(-1) != 1 or _overlaps_itself(t):
                     raise ValueError("inplace needs tensors with contiguous rows whose elements do not share memory")
-            if len(tensors) == 2 and tensors[0].untyped_storage().data_ptr() == tensors[1].untyped_storage().data_ptr() \
-                    and tensors[0].data_ptr() == tensors[1].data_ptr():
+            if len(tensors) == 2 and tensors[0].data_ptr() == tensors[1].data_ptr() and tensors[0].numel() > 0:
                 raise ValueError("inplace needs two different tensors")
             src = outs = tuple(tensors)
         else:
-            src = tuple(t if t.stride(-1) == 1 else t.contiguous() for t in tensors)
-            outs = tuple(torch.empty(t.shape, dtype=t.dtype, device=t.device) for t in src)
-        x = src[0]
-        if x.shape[0] == 0 or x.shape[1] == 0:
+            src = tuple(t if t.stride(3) == 1 else t.contiguous() for t in tensors)
+            outs = tuple(torch.empty_like(t, requires_grad=False) for t in src)
+        x, y = src[0], outs[0]
+        B, L, H = x.shape[:3]
+        if B == 0 or L == 0:
             return outs
-        a = _lib.RotaryArgs()
-        for i, (t, o) in enumerate(zip(src, outs)):
-            a.x[i], a.y[i], a.H[i] = t.data_ptr(), o.data_ptr(), t.shape[2]
-            for d in range(3):
-                a.x_stride[i][d], a.y_stride[i][d] = t.stride(d), o.stride(d)
-        a.positions, a.pos64 = p.data_ptr(), int(p.dtype == torch.int64)
-        for d in range(3):
-            a.p_stride[d] = p.stride(d)
-        a.turns, a.axis = self._turns, self._axis
-        a.B, a.L, a.D = x.shape[0], x.shape[1], self.head_dim
-        a.n_pairs, a.n_axes, a.layout = len(self.frequencies), len(self.axis_pairs), int(self.layout == "half")
-        a.inverse, a.dtype, a.magnitude = int(inverse), _DTYPES[x.dtype], self.magnitude
-        with torch.cuda.device(x.device):
-            _lib.launch("mcs_rotary", a, x.device, "mcs_rotary")
+        xs, ys = x.stride(), y.stride()
+        if len(src) == 2:
+            x1, y1 = src[1], outs[1]
+            second = (x1.data_ptr(), y1.data_ptr(), x1.stride(), y1.stride(), x1.shape[2])
+        else:
+            second = (0, 0, (0, 0, 0, 0), (0, 0, 0, 0), 0)
+        xs1, ys1 = second[2], second[3]
+        a = _lib.packed(_lib.RotaryArgs, _ARGS, x.data_ptr(), second[0], y.data_ptr(), second[1],
+                        xs[0], xs[1], xs[2], xs1[0], xs1[1], xs1[2], ys[0], ys[1], ys[2], ys1[0], ys1[1], ys1[2],
+                        positions.data_ptr(), *p_stride, C.addressof(self._turns), C.addressof(self._axis),
+                        H, second[4], B, L, self.head_dim, len(self.frequencies), len(self.axis_pairs), int(self.layout == "half"),
+                        int(positions.dtype == torch.int64), int(inverse), _DTYPES[x.dtype], self.magnitude)
+        device = x.device
+        if device.index == torch.cuda.current_device():
+            _lib.launch("mcs_rotary", a, device, "mcs_rotary")
+        else:
+            with torch.cuda.device(device):
+                _lib.launch("mcs_rotary", a, device, "mcs_rotary")
         return outs
 
     def rotate(self, *tensors: Tensor, positions: Tensor, inplace: bool = False):
@@ -179,17 +193,15 @@ class RotaryEmbedding:
             self._check(tensors, positions)
             outs = _Rotate.apply(self, positions, *tensors)
         else:
-            outs = self._launch([t.detach() for t in tensors], positions, False, inplace)
-            if inplace:
-                outs = tensors
-        return outs[0] if len(tensors) == 1 else tuple(outs)
+            outs = self._launch(tensors, positions, False, inplace)
+        return outs[0] if len(tensors) == 1 else outs
 
     __call__ = rotate
 
     def rotate_backward(self, *grads: Tensor, positions: Tensor, inplace: bool = False):
         """Gradients of the rotated tensors' inputs from those of the outputs: the rotation the other way, same magnitude."""
-        outs = self._launch([g.detach() for g in grads], positions, True, inplace)
-        return outs[0] if len(grads) == 1 else tuple(outs)
+        outs = self._launch(grads, positions, True, inplace)
+        return outs[0] if len(grads) == 1 else outs
 
 
 def _overlaps_itself(t: Tensor) -> bool:
@@ -207,7 +219,7 @@ class _Rotate(torch.autograd.Function):
     def forward(ctx, plan: RotaryEmbedding, positions: Tensor, *tensors: Tensor):
         ctx.plan = plan
         ctx.save_for_backward(positions)
-        return plan._launch([t.detach() for t in tensors], positions, False, False)
+        return plan._launch(tensors, positions, False, False)
 
     @staticmethod
     @torch.autograd.function.once_differentiable
