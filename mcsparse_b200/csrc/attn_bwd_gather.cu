@@ -111,7 +111,8 @@ __global__ void __launch_bounds__(1024) attn_bwd_rows_kernel(const AttnBwdParams
 // One CTA per SM walks groups.  Q and dO of the group stay in shared memory; gathered K and V tiles of 128 keys come through a ring in
 // blocks of up to 128 columns.  Per tile:
 //     S^T = K Q^T, dP^T = V dO^T (rows: gathered keys)  ->  P^T, dS^T in tensor memory, over their scores
-//     dV = P^T dO, dK = dS^T Q, up to 128 columns at a time, copied to the entries' rows by the warps that computed P and dS
+//     dV = P^T dO, dK = dS^T Q, up to 128 columns at a time, copied to the entries' rows by four warps of their own
+// The copy is the longest part of a tile (128 D x 8 bytes through the SM's store path); the next tile's P and dS are computed under it.
 template <int DB>
 struct SmemG {
   static constexpr int kResBytes = DB * 16384;
@@ -120,8 +121,8 @@ struct SmemG {
   static constexpr int kRing = DB > 2 ? 2 : (DB == 2 ? 4 : 8);
   static constexpr int kQ = 0, kDO = kResBytes, kRingOff = 2 * kResBytes;
   static constexpr int kStat = kRingOff + kRing * kSlotBytes;               // neg_lse2, neg_delta of the group's rows
-  static constexpr int kStage = kStat + 1024;                               // 32 rows x 128 bytes of every softmax warp
-  static constexpr int kBars = kStage + 8 * 4096;
+  static constexpr int kStage = kStat + 1024;                               // 32 rows x 128 bytes of every copying warp
+  static constexpr int kBars = kStage + 4 * 4096;
   static constexpr int kFull = 0, kEmpty = kRing, kAFull = 2 * kRing, kAEmpty = kAFull + 1, kSFull = kAEmpty + 1, kDPFull = kSFull + 1,
                        kPReady = kDPFull + 1, kDSReady = kPReady + 1, kOFull = kDSReady + 1, kOFree = kOFull + 1, kDrain = kOFree + 1, kCount = kDrain + 1;
   static constexpr int kSlot = kBars + kCount * 8;
@@ -129,8 +130,8 @@ struct SmemG {
 };
 static_assert(SmemG<1>::kDynamic <= 232448 && SmemG<2>::kDynamic <= 232448 && SmemG<4>::kDynamic <= 232448, "must fit 227 KB");
 
-constexpr int kThreadsG = 480;                               // 8 softmax warps, the issuer, two resident copies, four producers
-constexpr int kIssueWarp = 8, kLoadWarp0 = 9, kRingWarp0 = 11;
+constexpr int kThreadsG = 512;                               // 8 softmax warps, the issuer, three producers, four warps that copy out
+constexpr int kIssueWarp = 8, kLoadWarp0 = 9, kLoadWarps = 3, kOutWarp0 = 12;
 constexpr uint32_t kColS = 0, kColDP = 128, kColDV = 256, kColDK = 384;
 
 template <int DB, bool kFp16>
@@ -166,14 +167,14 @@ __global__ void __launch_bounds__(kThreadsG, 1) attn_bwd_gather_dkv_kernel(const
 
   if (tid == 0) {
     for (int i = 0; i < R; ++i) { mbar_init(bar(L::kFull + i), 128); mbar_init(bar(L::kEmpty + i), 1); }
-    mbar_init(bar(L::kAFull), 64);
+    mbar_init(bar(L::kAFull), 256);
     mbar_init(bar(L::kAEmpty), 1);
     mbar_init(bar(L::kSFull), 1);
     mbar_init(bar(L::kDPFull), 1);
     mbar_init(bar(L::kPReady), kSoftmaxWarps);
     mbar_init(bar(L::kDSReady), kSoftmaxWarps);
     mbar_init(bar(L::kOFull), 1);
-    mbar_init(bar(L::kOFree), kSoftmaxWarps);
+    mbar_init(bar(L::kOFree), 4);
     mbar_init(bar(L::kDrain), 1);
     mbar_fence_init();
   }
@@ -191,31 +192,23 @@ __global__ void __launch_bounds__(kThreadsG, 1) attn_bwd_gather_dkv_kernel(const
       __syncwarp();
       if (lane == 0) mbar_arrive(b);
     };
-    const int x = warp >> 2, r_in = (warp & 3) * 32 + lane;
+    const int x = warp >> 2;
     const uint32_t lane_addr = (static_cast<uint32_t>(warp & 3) * 32u) << 16;
     const uint32_t tS = tmem + kColS + x * 64 + lane_addr, tDP = tmem + kColDP + x * 64 + lane_addr;
-    const uint32_t tO = tmem + (x == 0 ? kColDV : kColDK) + lane_addr;
     const unsigned long long scale2 = f2_pack(p.scale_log2, p.scale_log2);
     const ulonglong2* lse = reinterpret_cast<const ulonglong2*>(smem + L::kStat + x * 256);
     const ulonglong2* dlt = reinterpret_cast<const ulonglong2*>(smem + L::kStat + 512 + x * 256);
-    const float unbias = kFp16 ? 6.103515625e-05f : 1.f;                       // 2^-14
-    const uint32_t stage = s_base + L::kStage + warp * 4096;
-    int g = 0, ic = 0, blk = 0;
+    int g = 0, ic = 0;
     bool ok = true;
 #pragma unroll 1
     for (int item = blockIdx.x; item < n_items && ok; item += gridDim.x, ++ic) {
       const Item it = decode(item);
       const float c = ds_scale<kFp16>(p, it.bh);
       const unsigned long long c2 = f2_pack(c, c);
-      const float w = x == 0 ? unbias : p.out_scale / c * unbias;
-      const int32_t* rows = p.entry_row + ((size_t)it.bh * p.M + it.m) * p.gather_len + r_in;
-      // dK at columns [0, D) of a row, dV behind it
-      float* base = p.parts + (size_t)(it.bh - p.bh0) * p.M * p.gather_len * (2 * p.D) + (x == 0 ? p.D : 0);
       ok = mbar_wait(bar(L::kAFull), ic & 1, p.status, 150);
       if (!ok) break;
 #pragma unroll 1
       for (int t = 0; t < it.T; ++t, ++g) {
-        const int dst_row = rows[t * 128];
         ok = mbar_wait(bar(L::kSFull), g & 1, p.status, 151);
         if (!ok) break;
         tc_fence_after();
@@ -266,45 +259,6 @@ __global__ void __launch_bounds__(kThreadsG, 1) attn_bwd_gather_dkv_kernel(const
         tmem_wait_st();
         tc_fence_before();
         warp_arrive(bar(L::kDSReady));
-        // ---- the tile's dV (first half of the warps) and dK rows, 32 columns at a time through shared memory (16-byte chunks
-        // swizzled by row), so that eight lanes store 128 contiguous bytes: with each lane storing its own row, a store touched 32
-        // lines and this loop took the launch from 2.6 to 4.8 ms (24 heads x 256 groups x 2,048 keys x 128)
-        int to[8];
-#pragma unroll
-        for (int i = 0; i < 8; ++i) to[i] = __shfl_sync(0xffffffffu, dst_row, i * 4 + (lane >> 3));
-#pragma unroll 1
-        for (int cb = 0; cb < CB && ok; ++cb, ++blk) {
-          ok = mbar_wait(bar(L::kOFull), blk & 1, p.status, 153);
-          if (!ok) break;
-          tc_fence_after();
-          const int cols = min(128, p.D - cb * 128);
-#pragma unroll 1
-          for (int cc = 0; cc < cols; cc += 32) {
-            uint32_t r[32];
-            tmem_ld32(tO + cc, r);
-            tmem_wait_ld();
-            __syncwarp();                                    // the last block has been read out
-#pragma unroll
-            for (int q = 0; q < 8; ++q)
-              sts_v4(stage + lane * 128 + ((q ^ (lane & 7)) << 4),
-                     make_uint4(__float_as_uint(__uint_as_float(r[4 * q]) * w), __float_as_uint(__uint_as_float(r[4 * q + 1]) * w),
-                                __float_as_uint(__uint_as_float(r[4 * q + 2]) * w), __float_as_uint(__uint_as_float(r[4 * q + 3]) * w)));
-            __syncwarp();
-            const int q = lane & 7;
-            if (cc + q * 4 < cols) {
-              float* dst = base + cb * 128 + cc + q * 4;
-#pragma unroll
-              for (int i = 0; i < 8; ++i) {
-                const int rl = i * 4 + (lane >> 3);
-                const uint4 v = lds_v4(stage + rl * 128 + ((q ^ (rl & 7)) << 4));
-                __stcs(reinterpret_cast<uint4*>(dst + (size_t)to[i] * (2 * p.D)), v);
-              }
-            }
-          }
-          tc_fence_before();
-          warp_arrive(bar(L::kOFree));
-        }
-        if (!ok) break;
       }
     }
     tc_fence_before();
@@ -387,56 +341,130 @@ __global__ void __launch_bounds__(kThreadsG, 1) attn_bwd_gather_dkv_kernel(const
     }
     __syncwarp();
     tc_fence_before();
-  } else if (warp < kRingWarp0) {
-    // ---- Q with its lse (first warp), dO with its delta (second)
-    const bool is_do = warp != kLoadWarp0;
-    const void* src = is_do ? p.dout : p.q;
-    const int64_t* st = is_do ? p.dout_stride : p.q_stride;
-    int ic = 0;
+  } else if (warp < kOutWarp0) {
+    // ---- gathered rows, K blocks, then V blocks, of every tile: the warps take batches of 32 rows in turn.  Q, dO and their
+    // statistics follow the first block, which does not have to wait for the item before to be done with them.
+    const int w = warp - kLoadWarp0;
+    int n = 0, ic = 0, batch = 0;
     bool ok = true;
+    int key[4], next[4];                                     // indices of the tile that is copied, and of the next one, in flight meanwhile
+    auto fetch = [&](const int32_t* gi, int t, int (&dst)[4]) {
+#pragma unroll
+      for (int q = 0; q < 4; ++q) dst[q] = __ldg(gi + t * 128 + q * 32 + lane);
+    };
 #pragma unroll 1
     for (int item = blockIdx.x; item < n_items && ok; item += gridDim.x, ++ic) {
-      const Item it = decode(item);
-      if (ic > 0) ok = mbar_wait(bar(L::kAEmpty), (ic - 1) & 1, p.status, 160);
-      if (!ok) break;
-#pragma unroll 1
-      for (int q = 0; q < 4; ++q)
-        warp_copy_rows<DB>(s_base + (is_do ? L::kDO : L::kQ), 128, q * 32, row_of(it, q * 32 + lane), p.D,
-                           reinterpret_cast<const uint8_t*>(src) + 2 * ((size_t)it.b * st[0] + (size_t)it.h * st[2]), 2 * (size_t)st[1], src);
-      cp_async16(s_base + L::kStat + (is_do ? 512 : 0) + lane * 16, (is_do ? p.neg_delta_kv : p.neg_lse2) + ((size_t)it.bh * p.M + it.m) * 128 + lane * 4);
-      cp_async_arrive_noinc(bar(L::kAFull));
-    }
-    cp_async_wait_all();
-    tc_fence_before();
-  } else {
-    // ---- gathered rows: K blocks, then V blocks, of every tile
-    const int w = warp - kRingWarp0;
-    int n = 0;
-    bool ok = true;
-#pragma unroll 1
-    for (int item = blockIdx.x; item < n_items && ok; item += gridDim.x) {
       const Item it = decode(item);
       const int32_t* gi = p.gi + ((size_t)it.bh * p.M + it.m) * p.gather_len;
       const uint8_t* kb = reinterpret_cast<const uint8_t*>(p.k) + 2 * ((size_t)it.b * p.k_stride[0] + (size_t)it.h * p.k_stride[2]);
       const uint8_t* vb = reinterpret_cast<const uint8_t*>(p.v) + 2 * ((size_t)it.b * p.v_stride[0] + (size_t)it.h * p.v_stride[2]);
-      int next = __ldg(gi + w * 32 + lane);
+      fetch(gi, 0, key);
 #pragma unroll 1
       for (int t = 0; t < it.T && ok; ++t) {
-        const int mine = min(max(next, 0), p.Sk - 1);
-        if (t + 1 < it.T) next = __ldg(gi + (t + 1) * 128 + w * 32 + lane);          // in flight while this tile is copied
+        if (t + 1 < it.T) fetch(gi, t + 1, next);
 #pragma unroll 1
         for (int e = 0; e < 2 * CB; ++e, ++n) {
           const bool is_v = e >= CB;
           const int cb = is_v ? e - CB : e, slot = n % R;
           if (n >= R) ok = mbar_wait(bar(L::kEmpty + slot), (n / R - 1) & 1, p.status, 161);
           if (!ok) break;
-          warp_copy_rows<SB>(sRing(slot), 128, w * 32, mine, min(SB * 64, p.D - cb * 128), (is_v ? vb : kb) + cb * 256,
-                             2 * (size_t)(is_v ? p.v_stride[1] : p.k_stride[1]), p.k);
-          cp_async_arrive_noinc(bar(L::kFull + slot));
+#pragma unroll
+          for (int q = 0; q < 4; ++q) {
+            if (batch == w) {
+              warp_copy_rows<SB>(sRing(slot), 128, q * 32, min(max(key[q], 0), p.Sk - 1), min(SB * 64, p.D - cb * 128), (is_v ? vb : kb) + cb * 256,
+                                 2 * (size_t)(is_v ? p.v_stride[1] : p.k_stride[1]), p.k);
+              cp_async_arrive_noinc(bar(L::kFull + slot));
+            }
+            batch = batch == kLoadWarps - 1 ? 0 : batch + 1;
+          }
+          if (t == 0 && e == 0) {
+            if (ic > 0) ok = mbar_wait(bar(L::kAEmpty), (ic - 1) & 1, p.status, 160);
+            if (!ok) break;
+#pragma unroll 1
+            for (int q = 0; q < 8; ++q) {
+              if (batch == w) {
+                const bool is_do = q >= 4;
+                const int64_t* st = is_do ? p.dout_stride : p.q_stride;
+                const uint8_t* src = reinterpret_cast<const uint8_t*>(is_do ? p.dout : p.q) + 2 * ((size_t)it.b * st[0] + (size_t)it.h * st[2]);
+                warp_copy_rows<DB>(s_base + (is_do ? L::kDO : L::kQ), 128, (q & 3) * 32, row_of(it, (q & 3) * 32 + lane), p.D, src, 2 * (size_t)st[1], p.q);
+                if ((q & 3) == 0)
+                  cp_async16(s_base + L::kStat + (is_do ? 512 : 0) + lane * 16,
+                             (is_do ? p.neg_delta_kv : p.neg_lse2) + ((size_t)it.bh * p.M + it.m) * 128 + lane * 4);
+                cp_async_arrive_noinc(bar(L::kAFull));
+              }
+              batch = batch == kLoadWarps - 1 ? 0 : batch + 1;
+            }
+          }
         }
+#pragma unroll
+        for (int q = 0; q < 4; ++q) key[q] = next[q];
       }
     }
     cp_async_wait_all();
+    tc_fence_before();
+  } else {
+    // ---- dV and dK rows of every tile to their entries' rows, 32 columns at a time through shared memory (16-byte chunks swizzled by
+    // row), so that eight lanes store 128 contiguous bytes: with each lane storing its own row, a store touched 32 lines
+    const int lg = warp & 3;
+    const uint32_t lane_addr = (static_cast<uint32_t>(lg) * 32u) << 16;
+    const uint32_t stage = s_base + L::kStage + lg * 4096;
+    const float unbias = kFp16 ? 6.103515625e-05f : 1.f;                       // 2^-14
+    int blk = 0;
+    bool ok = true;
+#pragma unroll 1
+    for (int item = blockIdx.x; item < n_items && ok; item += gridDim.x) {
+      const Item it = decode(item);
+      const float w_k = p.out_scale / ds_scale<kFp16>(p, it.bh) * unbias;
+      const int32_t* rows = p.entry_row + ((size_t)it.bh * p.M + it.m) * p.gather_len + lg * 32 + lane;
+      // dK at columns [0, D) of a row, dV behind it
+      float* base = p.parts + (size_t)(it.bh - p.bh0) * p.M * p.gather_len * (2 * p.D) + (lane & 7) * 4;
+      int next = rows[0];
+#pragma unroll 1
+      for (int t = 0; t < it.T && ok; ++t) {
+        const int mine = next;
+        if (t + 1 < it.T) next = rows[(t + 1) * 128];
+        int to[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) to[i] = __shfl_sync(0xffffffffu, mine, i * 4 + (lane >> 3));
+#pragma unroll 1
+        for (int cb = 0; cb < CB; ++cb, ++blk) {
+          ok = mbar_wait(bar(L::kOFull), blk & 1, p.status, 153);
+          if (!ok) break;
+          tc_fence_after();
+          const int cols = min(128, p.D - cb * 128);
+#pragma unroll 1
+          for (int part = 0; part < 2; ++part) {
+            const float w = part == 0 ? unbias : w_k;
+            float* to_cols = base + (part == 0 ? p.D : 0) + cb * 128;
+            const uint32_t tO = tmem + (part == 0 ? kColDV : kColDK) + lane_addr;
+#pragma unroll 1
+            for (int cc = 0; cc < cols; cc += 32) {
+              uint32_t r[32];
+              tmem_ld32(tO + cc, r);
+              tmem_wait_ld();
+              __syncwarp();                                  // the last block has been read out
+#pragma unroll
+              for (int q = 0; q < 8; ++q)
+                sts_v4(stage + lane * 128 + ((q ^ (lane & 7)) << 4),
+                       make_uint4(__float_as_uint(__uint_as_float(r[4 * q]) * w), __float_as_uint(__uint_as_float(r[4 * q + 1]) * w),
+                                  __float_as_uint(__uint_as_float(r[4 * q + 2]) * w), __float_as_uint(__uint_as_float(r[4 * q + 3]) * w)));
+              __syncwarp();
+              if (cc + (lane & 7) * 4 < cols) {
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                  const int rl = i * 4 + (lane >> 3);
+                  const uint4 v = lds_v4(stage + rl * 128 + (((lane & 7) ^ (rl & 7)) << 4));
+                  *reinterpret_cast<uint4*>(to_cols + (size_t)to[i] * (2 * p.D) + cc) = v;
+                }
+              }
+            }
+          }
+          __syncwarp();
+          tc_fence_before();
+          if (lane == 0) mbar_arrive(bar(L::kOFree));
+        }
+      }
+    }
     tc_fence_before();
   }
 
