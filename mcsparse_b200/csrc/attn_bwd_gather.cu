@@ -124,7 +124,7 @@ struct SmemG {
   static constexpr int kStage = kStat + 1024;                               // 32 rows x 128 bytes of every copying warp
   static constexpr int kBars = kStage + 4 * 4096;
   static constexpr int kFull = 0, kEmpty = kRing, kAFull = 2 * kRing, kAEmpty = kAFull + 1, kSFull = kAEmpty + 1, kDPFull = kSFull + 1,
-                       kPReady = kDPFull + 1, kDSReady = kPReady + 1, kOFull = kDSReady + 1, kOFree = kOFull + 1, kDrain = kOFree + 1, kCount = kDrain + 1;
+                       kPReady = kDPFull + 1, kDSReady = kPReady + 1, kOFull = kDSReady + 1, kOFree = kOFull + 2, kDrain = kOFree + 2, kCount = kDrain + 1;   // kOFull, kOFree: dV, dK
   static constexpr int kSlot = kBars + kCount * 8;
   static constexpr int kDynamic = kSlot + 16 + 1024;
 };
@@ -173,8 +173,7 @@ __global__ void __launch_bounds__(kThreadsG, 1) attn_bwd_gather_dkv_kernel(const
     mbar_init(bar(L::kDPFull), 1);
     mbar_init(bar(L::kPReady), kSoftmaxWarps);
     mbar_init(bar(L::kDSReady), kSoftmaxWarps);
-    mbar_init(bar(L::kOFull), 1);
-    mbar_init(bar(L::kOFree), 4);
+    for (int i = 0; i < 2; ++i) { mbar_init(bar(L::kOFull + i), 1); mbar_init(bar(L::kOFree + i), 4); }
     mbar_init(bar(L::kDrain), 1);
     mbar_fence_init();
   }
@@ -311,11 +310,13 @@ __global__ void __launch_bounds__(kThreadsG, 1) attn_bwd_gather_dkv_kernel(const
         if (!ok) break;
         tc_fence_after();
         out_product(tmem + kColDV, tmem + kColS, s_base + L::kDO, 0);
+        if (leader) tc_commit(bar(L::kOFull));
         ok = mbar_wait(bar(L::kDSReady), g & 1, p.status, 158);
+        if (ok && blk > 0) ok = mbar_wait(bar(L::kOFree + 1), (blk - 1) & 1, p.status, 162);
         if (!ok) break;
         tc_fence_after();
         out_product(tmem + kColDK, tmem + kColDP, s_base + L::kQ, 0);
-        if (leader) tc_commit(bar(L::kOFull));
+        if (leader) tc_commit(bar(L::kOFull + 1));
         ++blk;
 #pragma unroll 1
         for (int cb = 1; cb < CB; ++cb, ++blk) {
@@ -323,8 +324,12 @@ __global__ void __launch_bounds__(kThreadsG, 1) attn_bwd_gather_dkv_kernel(const
           if (!ok) break;
           tc_fence_after();
           out_product(tmem + kColDV, tmem + kColS, s_base + L::kDO, cb);
-          out_product(tmem + kColDK, tmem + kColDP, s_base + L::kQ, cb);
           if (leader) tc_commit(bar(L::kOFull));
+          ok = mbar_wait(bar(L::kOFree + 1), (blk - 1) & 1, p.status, 162);
+          if (!ok) break;
+          tc_fence_after();
+          out_product(tmem + kColDK, tmem + kColDP, s_base + L::kQ, cb);
+          if (leader) tc_commit(bar(L::kOFull + 1));
         }
         if (!ok) break;
         if (t + 1 < it.T) {
@@ -428,12 +433,13 @@ __global__ void __launch_bounds__(kThreadsG, 1) attn_bwd_gather_dkv_kernel(const
         for (int i = 0; i < 8; ++i) to[i] = __shfl_sync(0xffffffffu, mine, i * 4 + (lane >> 3));
 #pragma unroll 1
         for (int cb = 0; cb < CB; ++cb, ++blk) {
-          ok = mbar_wait(bar(L::kOFull), blk & 1, p.status, 153);
-          if (!ok) break;
-          tc_fence_after();
           const int cols = min(128, p.D - cb * 128);
+          // (dV of the next tile is computed while this one's dK is copied)
 #pragma unroll 1
           for (int part = 0; part < 2; ++part) {
+            ok = ok && mbar_wait(bar(L::kOFull + part), blk & 1, p.status, 153);
+            if (!ok) break;
+            tc_fence_after();
             const float w = part == 0 ? unbias : w_k;
             float* to_cols = base + (part == 0 ? p.D : 0) + cb * 128;
             const uint32_t tO = tmem + (part == 0 ? kColDV : kColDK) + lane_addr;
@@ -458,10 +464,11 @@ __global__ void __launch_bounds__(kThreadsG, 1) attn_bwd_gather_dkv_kernel(const
                 }
               }
             }
+            __syncwarp();
+            tc_fence_before();
+            if (lane == 0) mbar_arrive(bar(L::kOFree + part));
           }
-          __syncwarp();
-          tc_fence_before();
-          if (lane == 0) mbar_arrive(bar(L::kOFree));
+          if (!ok) break;
         }
       }
     }
