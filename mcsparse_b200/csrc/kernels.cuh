@@ -167,7 +167,7 @@ struct RotaryParams {
   unsigned char axis[kRotaryMaxPairs];
   int B, L, D, n_pairs, pos64, inverse;
   float magnitude;
-  int units, rot_units, unit_threads, tokens_per_cta, heads_per_cta;   // set by the launch
+  int units, rot_units, tokens_per_cta, heads_per_cta;   // set by the launch
 };
 int launch_rotary(RotaryParams& p, int type, bool half, cudaStream_t stream);
 

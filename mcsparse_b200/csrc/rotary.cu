@@ -109,19 +109,22 @@ __device__ __forceinline__ void walk_heads(const typename Elem<kType>::T* x, typ
   }
 }
 
-// A CTA takes `tokens_per_cta` tokens with `unit_threads` threads each; blockIdx.y is a run of heads of q and k together.
+// A CTA takes `tokens_per_cta` tokens: their rotated units first, then the units that are copied, so that few warps do both.
+// blockIdx.y is a run of heads of q and k together.
 template <int kType, bool kHalf, int kVec>
 __global__ void __launch_bounds__(kThreadsR) rotary_kernel(const __grid_constant__ RotaryParams p) {
   using Y = Layout<kType, kHalf, kVec>;
   using T = typename Y::T;
   constexpr int kPairs = Y::kPairs;
-  const int sub = threadIdx.x / p.unit_threads, lane = threadIdx.x - sub * p.unit_threads;
-  const long long token = (long long)blockIdx.x * p.tokens_per_cta + sub;
-  if (sub >= p.tokens_per_cta || token >= (long long)p.B * p.L) return;
-  const int b = (int)(token / p.L), row = (int)(token - (long long)b * p.L);
   const int h0 = blockIdx.y * p.heads_per_cta, h1 = min(h0 + p.heads_per_cta, p.H[0] + p.H[1]);
-  for (int unit = lane; unit < p.units; unit += p.unit_threads) {
-    const bool rotates = unit < p.rot_units;
+  const int turning = p.tokens_per_cta * p.rot_units, copied = p.units - p.rot_units;
+  for (int i = threadIdx.x; i < p.tokens_per_cta * p.units; i += kThreadsR) {
+    const bool rotates = i < turning;
+    const int n = rotates ? p.rot_units : copied, at = rotates ? i : i - turning, sub = at / n;
+    const int unit = (rotates ? 0 : p.rot_units) + at - sub * n;
+    const long long token = (long long)blockIdx.x * p.tokens_per_cta + sub;
+    if (token >= (long long)p.B * p.L) continue;
+    const int b = (int)(token / p.L), row = (int)(token - (long long)b * p.L);
     float c[kPairs], s[kPairs];
     if (rotates) {
       const long long base = b * p.p_stride[0] + row * p.p_stride[1];
@@ -158,16 +161,16 @@ int launch_variant(RotaryParams& p, bool copy_rest, cudaStream_t stream) {
   p.rot_units = p.n_pairs / Layout<kType, kHalf, kVec>::kPairs;
   p.units = p.rot_units + (copy_rest ? (p.D - 2 * p.n_pairs) / kVec : 0);
   if (p.units == 0) return 0;
-  p.unit_threads = p.units < kThreadsR ? p.units : kThreadsR;
-  p.tokens_per_cta = kThreadsR / p.unit_threads;
+  p.tokens_per_cta = p.units < kThreadsR ? kThreadsR / p.units : 1;
   const int heads = p.H[0] + p.H[1];
   const long long tokens = (long long)p.B * p.L, ctas = (tokens + p.tokens_per_cta - 1) / p.tokens_per_cta;
   if (ctas > 0x7fffffffLL) return -10;
-  // Up to kMaxHeads heads share one computation of the angles; with few tokens a CTA takes fewer, so that the launch still
-  // fills the GPU (148 SMs x 8 CTAs).
+  // Up to kMaxHeads heads share one computation of the angles; a CTA takes fewer, eight at least, where that leaves four waves of
+  // 148 x 8 CTAs or less, and single heads where the launch would not fill the GPU (one new token: latency is all).
   constexpr int kMaxHeads = 16;
-  long long per = ctas * heads / (148 * 8);
-  per = per < 1 ? 1 : (per > kMaxHeads ? kMaxHeads : per);
+  long long per = ctas * heads / (148 * 8 * 4);
+  per = per > kMaxHeads ? kMaxHeads : (per < 8 ? 8 : per / 4 * 4);
+  if (ctas * ((heads + per - 1) / per) < 148 * 8) per = 1;
   if ((heads + per - 1) / per > 65535) per = (heads + 65534) / 65535;
   p.heads_per_cta = (int)per;
   rotary_kernel<kType, kHalf, kVec><<<dim3((unsigned)ctas, (unsigned)((heads + per - 1) / per)), kThreadsR, 0, stream>>>(p);
