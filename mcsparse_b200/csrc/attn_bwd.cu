@@ -43,7 +43,7 @@ __global__ void __launch_bounds__(256) attn_bwd_stats_kernel(const AttnBwdParams
   constexpr int kRows = 4;
   const int bh = blockIdx.y, h = bh % p.H, b = bh / p.H;
   const int l16 = threadIdx.x & 15, sub = threadIdx.x >> 4;
-  const int rows = p.M * 128;
+  const int rows = p.stat_rows;
   const int chunks = p.D / 8;
   const uint8_t* gb = reinterpret_cast<const uint8_t*>(p.dout) + 2 * ((size_t)b * p.dout_stride[0] + (size_t)h * p.dout_stride[2]);
   const uint8_t* ob = reinterpret_cast<const uint8_t*>(p.out) + 2 * ((size_t)b * p.out_stride[0] + (size_t)h * p.out_stride[2]);
@@ -173,14 +173,16 @@ constexpr bool fits = SmemB<DB, TN>::kDynamic <= kMaxSmem && SmemB<DB, TN>::kCol
 static_assert(fits<1, 128> && fits<2, 128> && fits<3, 64> && fits<4, 64>, "227 KB of shared memory, 512 columns of tensor memory");
 
 // Warps: eight softmax warps, the issuer, then for the dense modes the producers of the resident tiles and of the ring, for gathered keys
-// three warps that copy both (a thirteenth warp would leave 128 registers each instead of 168).
-constexpr int kIssueWarp = 8, kLoadWarp0 = 9, kThreadsB = 384;
+// seven warps that copy both: 512 threads of 128 registers.  (24 heads x 256 groups x 2,048 keys x 128: three warps, which leave 168
+// registers, 1.63 ms, four 1.54, seven 1.48.)
+constexpr int kIssueWarp = 8, kLoadWarp0 = 9, kGatherWarps = 7;
+constexpr int threads_of(int mode) { return mode == kDqGather ? 32 * (kLoadWarp0 + kGatherWarps) : 384; }
 
 // Blocks of output columns: one, or two of 128 where tensor memory does not hold both sums at full width.
 __host__ __device__ constexpr int column_blocks(int D) { return D > 192 ? 2 : 1; }
 
 template <int DB, int TN, bool kFp16, int kMode>
-__global__ void __launch_bounds__(kThreadsB, 1) attn_bwd_kernel(const AttnBwdParams p, const __grid_constant__ DenseTileMaps maps,
+__global__ void __launch_bounds__(threads_of(kMode), 1) attn_bwd_kernel(const AttnBwdParams p, const __grid_constant__ DenseTileMaps maps,
                                                                 const __grid_constant__ DenseTileMaps res) {
   using L = SmemB<DB, TN>;
   using G = Geo<DB, TN>;
@@ -280,7 +282,7 @@ __global__ void __launch_bounds__(kThreadsB, 1) attn_bwd_kernel(const AttnBwdPar
       const unsigned long long c2 = f2_pack(c, c);
       unsigned long long nl2 = 0, nd2 = 0, rs[2] = {0, 0}, es[2] = {0, 0};   // kDq: this row's statistics, sums of its dS rounded and not
       if constexpr (!kRowsAreKeys) {
-        const size_t si = ((size_t)it.bh * p.M + it.m) * 128 + r_in;
+        const size_t si = (size_t)it.bh * p.stat_rows + it.m * 128 + r_in;
         const float nl = p.neg_lse2[si], ndl = p.neg_delta[si];
         nl2 = f2_pack(nl, nl);
         nd2 = f2_pack(ndl, ndl);
@@ -295,8 +297,7 @@ __global__ void __launch_bounds__(kThreadsB, 1) attn_bwd_kernel(const AttnBwdPar
         if (!ok) break;
         tc_fence_after();
         uint32_t sc[HC];
-#pragma unroll
-        for (int q = 0; q < HC / 32; ++q) tmem_ld32(tS + q * 32, *reinterpret_cast<uint32_t(*)[32]>(&sc[q * 32]));
+        load_columns<HC>(tS, sc);
         tmem_wait_ld();
         tc_fence_before();
         warp_arrive(bar(L::kSFree));
@@ -328,13 +329,12 @@ __global__ void __launch_bounds__(kThreadsB, 1) attn_bwd_kernel(const AttnBwdPar
         if constexpr (kRowsAreKeys) ok = ok && mbar_wait(bar(L::kFull + n1 % R), (n1 / R) & 1, p.status, 133);
         if (!ok) break;
         tc_fence_after();
-        // dP in steps of 32 columns, all in flight at once where the registers allow it; P goes over the first half of this thread's
-        // columns as soon as those are read, dS over the second half
-        constexpr int kSteps = HC / 32;
-        constexpr bool kAll = false;
-        uint32_t dp[kAll ? HC : 32], pk[HC / 2];
-        tmem_ld32(tDP, *reinterpret_cast<uint32_t(*)[32]>(&dp[0]));
-        if constexpr (kAll && kSteps == 2) tmem_ld32(tDP + 32, *reinterpret_cast<uint32_t(*)[32]>(&dp[kAll && kSteps == 2 ? 32 : 0]));
+        // dP in steps of 32 columns (all 64 at once would spill); P goes over the first half of this thread's columns as soon as
+        // those are read, dS over the second half
+        constexpr int kStep = 32;
+        static_assert(kStep >= HC / 2, "P overwrites columns that have been read");
+        uint32_t dp[kStep], pk[HC / 2];
+        load_columns<kStep>(tDP, dp);
         tmem_wait_ld();
 #pragma unroll
         for (int q = 0; q < HC / 16; ++q) store_packed<kFp16>(tDP + q * 8, &sc[q * 16]);
@@ -342,14 +342,14 @@ __global__ void __launch_bounds__(kThreadsB, 1) attn_bwd_kernel(const AttnBwdPar
         tc_fence_before();
         warp_arrive(bar(L::kPReady));
 #pragma unroll
-        for (int st = 0; st < kSteps; ++st) {
-          if (!kAll && st > 0) {
-            tmem_ld32(tDP + 32, *reinterpret_cast<uint32_t(*)[32]>(&dp[0]));
+        for (int s0 = 0; s0 < HC; s0 += kStep) {
+          if (s0 > 0) {
+            load_columns<kStep>(tDP + s0, dp);
             tmem_wait_ld();
           }
 #pragma unroll
-          for (int i = 0; i < 8; ++i) {
-            const int e = st * 32 + 4 * i, d = kAll ? e : 4 * i;
+          for (int d = 0; d < kStep; d += 4) {
+            const int e = s0 + d;
             unsigned long long e0 = nd2, e1 = nd2;
             if constexpr (kRowsAreKeys) {
               const ulonglong2 l = dlt[e / 4];
@@ -394,7 +394,7 @@ __global__ void __launch_bounds__(kThreadsB, 1) attn_bwd_kernel(const AttnBwdPar
         fix = sums[r_in] + sums[128 + r_in];
         off = (off + sums[256 + r_in]) * unbias / c;         // (used by the first half only)
         if (p.splits == 1 && x == 0 && it.c0 == 0) {
-          const size_t si = ((size_t)it.bh * p.M + it.m) * 128 + r_in;
+          const size_t si = (size_t)it.bh * p.stat_rows + it.m * 128 + r_in;
           p.neg_delta_kv[si] = p.neg_delta[si] - off;
         }
       }
@@ -561,7 +561,7 @@ __global__ void __launch_bounds__(kThreadsB, 1) attn_bwd_kernel(const AttnBwdPar
   } else if (kGather) {
     // ---- gathered keys: the warps take batches of 32 rows in turn.  The resident tiles of an item follow its first pair of T tiles,
     // which do not have to wait for the item before to be done with A0 and A1.
-    constexpr int kBatches = TN / 32, kWarps = 3;
+    constexpr int kBatches = TN / 32, kWarps = kGatherWarps;
     const int w = warp - kLoadWarp0;
     int n = 0, ic = 0, batch = 0;
     bool ok = true;
@@ -630,16 +630,13 @@ __global__ void __launch_bounds__(kThreadsB, 1) attn_bwd_kernel(const AttnBwdPar
       if (!ok) break;
       if (leader) {
         mbar_arrive_expect_tx(bar(L::kAFull), 2 * G::kResBytes);
+        int c0[4] = {0, 0, 0, 0}, c1[4] = {0, 0, 0, 0};
+        c0[res.k_pos_h] = it.h; c0[res.k_pos_b] = it.b; c0[res.k_pos_row] = it.m * 128;
+        c1[res.v_pos_h] = it.h; c1[res.v_pos_b] = it.b; c1[res.v_pos_row] = it.m * 128;
 #pragma unroll
-        for (int half = 0; half < 128 / TN; ++half) {
-          int c0[4] = {0, 0, 0, 0}, c1[4] = {0, 0, 0, 0};
-          c0[res.k_pos_h] = it.h; c0[res.k_pos_b] = it.b; c0[res.k_pos_row] = it.m * 128 + half * TN;
-          c1[res.v_pos_h] = it.h; c1[res.v_pos_b] = it.b; c1[res.v_pos_row] = it.m * 128 + half * TN;
-#pragma unroll
-          for (int cb = 0; cb < DB; ++cb) {
-            tma_load_4d(s_base + L::kA0 + cb * 16384 + half * TN * 128, res.k, cb * 64, c0[1], c0[2], c0[3], bar(L::kAFull));
-            tma_load_4d(s_base + L::kA1 + cb * 16384 + half * TN * 128, res.v, cb * 64, c1[1], c1[2], c1[3], bar(L::kAFull));
-          }
+        for (int cb = 0; cb < DB; ++cb) {
+          tma_load_4d(s_base + L::kA0 + cb * 16384, res.k, cb * 64, c0[1], c0[2], c0[3], bar(L::kAFull));
+          tma_load_4d(s_base + L::kA1 + cb * 16384, res.v, cb * 64, c1[1], c1[2], c1[3], bar(L::kAFull));
         }
       }
     }
@@ -671,7 +668,7 @@ __global__ void __launch_bounds__(kThreadsB, 1) attn_bwd_kernel(const AttnBwdPar
           for (int cb = 0; cb < DB; ++cb)
             tma_load_4d(sRing(slot) + cb * TN * 128, map, cb * 64, co[1], co[2], co[3], bar(L::kFull + slot));
           if constexpr (kRowsAreKeys)
-            bulk_load(s_base + L::kStat + slot * TN * 4, (is_t1 ? p.neg_delta_kv : p.neg_lse2) + (size_t)it.bh * p.M * 128 + (size_t)(e >> 1) * TN, TN * 4,
+            bulk_load(s_base + L::kStat + slot * TN * 4, (is_t1 ? p.neg_delta_kv : p.neg_lse2) + (size_t)it.bh * p.stat_rows + (size_t)(e >> 1) * TN, TN * 4,
                       bar(L::kFull + slot));
         }
       }
@@ -695,7 +692,7 @@ __global__ void __launch_bounds__(kThreadsB, 1) attn_bwd_kernel(const AttnBwdPar
 template <bool kFp16, bool kFix>
 __global__ void __launch_bounds__(256) attn_bwd_sum_kernel(const float* parts, int splits, long long split_pitch, int pitch, int col0, int D, int H, int S,
                                                            long long rows, void* out, long long sb, long long ss, long long sh,
-                                                           const float* neg_delta, float* neg_delta_kv) {
+                                                           const float* neg_delta, float* neg_delta_kv, int stat_rows) {
   const int chunks = D / 8;
   const long long n = rows * chunks;
   for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < n; i += (long long)gridDim.x * 256) {
@@ -719,7 +716,7 @@ __global__ void __launch_bounds__(256) attn_bwd_sum_kernel(const float* parts, i
       if (c == 0) {
         float off = 0.f;
         for (int s = 0; s < splits; ++s) off += base[2 * D + 1 + s * split_pitch];
-        const long long bh = row / S, si = bh * ((S + 127) / 128 * 128) + (row - bh * S);
+        const long long bh = row / S, si = bh * stat_rows + (row - bh * S);
         neg_delta_kv[si] = neg_delta[si] - off;
       }
 #pragma unroll
@@ -737,16 +734,18 @@ int sm_count() {
   return sms;
 }
 
-// Splits of the summed axis (T tiles) for `items` items without splits.  A launch takes waves of one item per SM; an item costs its
-// tiles and about two tiles' time to fill and drain.  Splits that do not end the launch earlier are not made: they cost the
-// partial sums' traffic.
-int pick_splits(long long items, int T, int sms) {
-  if (items >= 4LL * sms) return 1;
-  long long best = -1;
+// Splits of the summed axis (T tiles) for `items` items without splits, whose partial sums are `part_bytes` per split.  Measured
+// at 1.9 GHz: a tile takes tile_us; an item besides 3.5 us to fill, drain and store (5.5 us with fp32 partial sums); the kernel that
+// adds the partial sums reads them at 4.3 TB/s and costs 2.5 us to launch.
+int pick_splits(long long items, int T, double tile_us, double part_bytes) {
+  // (for the B200's 148 SMs, whatever the current device: the workspace must not depend on the device that asks)
+  constexpr int kSms = 148;
+  double best = 0;
   int pick = 1;
   for (int s = 1; s <= T && s <= 32; ++s) {
-    const long long cost = ((items * s + sms - 1) / sms) * ((T + s - 1) / s + 2) + (s > 1 ? 2 : 0);
-    if (best < 0 || cost < best) { best = cost; pick = s; }
+    const double waves = (double)((items * s + kSms - 1) / kSms);
+    const double us = waves * ((T + s - 1) / s * tile_us + (s > 1 ? 5.5 : 3.5)) + (s > 1 ? 2.5 + s * part_bytes / 4.3e6 : 0.0);
+    if (s == 1 || us < best) { best = us; pick = s; }
   }
   return pick;
 }
@@ -755,23 +754,32 @@ int pick_splits(long long items, int T, int sms) {
 // passes would only add launches with a partly filled last wave.
 constexpr size_t kPartsBytes = 4ull << 30;
 
-struct Plan { int dq_splits, kv_splits, segs, heads_per_pass; size_t stats, row_max, entries, starts, counts, blocks, parts, total; };
+struct Plan { int stat_rows, dq_splits, kv_splits, segs, heads_per_pass; size_t stats, row_max, entries, starts, counts, blocks, parts, total; };
 
 constexpr size_t kAlign = 256;
 size_t up(size_t n) { return (n + kAlign - 1) / kAlign * kAlign; }
 
+// Rows of a streamed tile: as many as tensor memory holds beside both sums, and shared memory beside the resident tiles.  (96 rows up to
+// D = 160 would fit, with a ring of three tiles instead of five: 18,944 x 144 took 488 us a side against 455.)
+int tile_rows(int D) { return D <= 128 ? 128 : 64; }
+
 int padded_blocks(int D) { return D <= 64 ? 1 : (D <= 128 ? 2 : (D <= 192 ? 3 : 4)); }
 
 Plan make_plan(const AttnBwdParams& p, bool gather) {
-  // (the split rule uses the B200's 148 SMs, not the current device's: sizes must not depend on the device that asks)
   constexpr int kSms = 148;
   Plan w{};
-  const int TN = padded_blocks(p.D) > 2 ? 64 : 128;
+  const int TN = tile_rows(p.D);
   const long long bh = (long long)p.B * p.H;
   const int blocks = column_blocks(p.D);
-  w.dq_splits = gather ? 1 : pick_splits(bh * p.M * blocks, (p.Sk + TN - 1) / TN, kSms);
-  w.kv_splits = gather ? 1 : pick_splits(bh * ((p.Sk + 127) / 128) * blocks, (p.Sq + TN - 1) / TN, kSms);
-  w.stats = up((size_t)bh * p.M * 128 * 4);
+  if (gather) {
+    w.dq_splits = w.kv_splits = 1;
+  } else {
+    const double tile_us = p.D <= 64 ? 1.5 : (p.D <= 128 ? 1.9 : 1.5);
+    w.dq_splits = pick_splits(bh * p.M * blocks, (p.Sk + TN - 1) / TN, tile_us, (double)bh * p.Sq * (2 * p.D + 8) * 4);
+    w.kv_splits = pick_splits(bh * ((p.Sk + 127) / 128) * blocks, (p.Sq + TN - 1) / TN, tile_us, (double)bh * p.Sk * 2 * p.D * 4);
+  }
+  w.stat_rows = p.M * 128;
+  w.stats = up((size_t)bh * w.stat_rows * 4);
   w.row_max = up((size_t)bh * kMaxBlocks * 8);
   size_t a = w.dq_splits > 1 ? (size_t)w.dq_splits * bh * p.Sq * (2 * p.D + 8) * 4 : 0, b = w.kv_splits > 1 ? (size_t)w.kv_splits * bh * p.Sk * 2 * p.D * 4 : 0;
   w.parts = up(a > b ? a : b);
@@ -803,12 +811,16 @@ int set_smem(K kern, int bytes) {
 
 template <int DB, int TN, bool kFp16>
 int launch_dense(AttnBwdParams& p, const Plan& w, cudaStream_t stream) {
-  DenseTileMaps kv, qd;
-  if (!encode_tile_map(p.k, p.k_stride, p.B, p.Sk, p.H, p.D, kv.k, kv.k_pos_h, kv.k_pos_row, kv.k_pos_b, TN) ||
-      !encode_tile_map(p.v, p.v_stride, p.B, p.Sk, p.H, p.D, kv.v, kv.v_pos_h, kv.v_pos_row, kv.v_pos_b, TN) ||
-      !encode_tile_map(p.q, p.q_stride, p.B, p.Sq, p.H, p.D, qd.k, qd.k_pos_h, qd.k_pos_row, qd.k_pos_b, TN) ||
-      !encode_tile_map(p.dout, p.dout_stride, p.B, p.Sq, p.H, p.D, qd.v, qd.v_pos_h, qd.v_pos_row, qd.v_pos_b, TN))
-    return -9;
+  // boxes of TN rows for streamed tiles, of 128 for resident ones
+  auto maps = [&](DenseTileMaps& m, const void* a, const int64_t* as, const void* b, const int64_t* bs, int S, int rows) {
+    return encode_tile_map(a, as, p.B, S, p.H, p.D, m.k, m.k_pos_h, m.k_pos_row, m.k_pos_b, rows) &&
+           encode_tile_map(b, bs, p.B, S, p.H, p.D, m.v, m.v_pos_h, m.v_pos_row, m.v_pos_b, rows);
+  };
+  DenseTileMaps kv, qd, res_kv, res_qd;
+  if (!maps(kv, p.k, p.k_stride, p.v, p.v_stride, p.Sk, TN) || !maps(qd, p.q, p.q_stride, p.dout, p.dout_stride, p.Sq, TN)) return -9;
+  res_kv = kv;
+  res_qd = qd;
+  if (TN != 128 && (!maps(res_kv, p.k, p.k_stride, p.v, p.v_stride, p.Sk, 128) || !maps(res_qd, p.q, p.q_stride, p.dout, p.dout_stride, p.Sq, 128))) return -9;
   const int sms = sm_count();
   const long long bh = (long long)p.B * p.H;
   auto dq = attn_bwd_kernel<DB, TN, kFp16, kDq>;
@@ -819,20 +831,20 @@ int launch_dense(AttnBwdParams& p, const Plan& w, cudaStream_t stream) {
   auto grid_of = [](long long n) { return (unsigned)(n / 256 + 1 < 148 * 8 ? n / 256 + 1 : 148 * 8); };
   p.splits = w.dq_splits;
   long long items = bh * p.M * blocks * p.splits;
-  dq<<<(unsigned)(items < sms ? items : sms), kThreadsB, kSmem, stream>>>(p, kv, qd);
+  dq<<<(unsigned)(items < sms ? items : sms), 384, kSmem, stream>>>(p, kv, res_qd);
   if (p.splits > 1)
     attn_bwd_sum_kernel<kFp16, true><<<grid_of(bh * p.Sq * (p.D / 8)), 256, 0, stream>>>(
         p.parts, p.splits, bh * p.Sq * (2 * p.D + 8), 2 * p.D + 8, 0, p.D, p.H, p.Sq, bh * p.Sq, p.dq, p.dq_stride[0], p.dq_stride[1], p.dq_stride[2],
-        p.neg_delta, p.neg_delta_kv);
+        p.neg_delta, p.neg_delta_kv, p.stat_rows);
   p.splits = w.kv_splits;
   items = bh * ((p.Sk + 127) / 128) * blocks * p.splits;
-  dkv<<<(unsigned)(items < sms ? items : sms), kThreadsB, kSmem, stream>>>(p, qd, kv);
+  dkv<<<(unsigned)(items < sms ? items : sms), 384, kSmem, stream>>>(p, qd, res_kv);
   if (p.splits > 1) {
     const unsigned grid = grid_of(bh * p.Sk * (p.D / 8));
     attn_bwd_sum_kernel<kFp16, false><<<grid, 256, 0, stream>>>(p.parts, p.splits, bh * p.Sk * 2 * p.D, 2 * p.D, 0, p.D, p.H, p.Sk, bh * p.Sk, p.dk,
-                                                                p.dk_stride[0], p.dk_stride[1], p.dk_stride[2], nullptr, nullptr);
+                                                                p.dk_stride[0], p.dk_stride[1], p.dk_stride[2], nullptr, nullptr, 0);
     attn_bwd_sum_kernel<kFp16, false><<<grid, 256, 0, stream>>>(p.parts, p.splits, bh * p.Sk * 2 * p.D, 2 * p.D, p.D, p.D, p.H, p.Sk, bh * p.Sk, p.dv,
-                                                                p.dv_stride[0], p.dv_stride[1], p.dv_stride[2], nullptr, nullptr);
+                                                                p.dv_stride[0], p.dv_stride[1], p.dv_stride[2], nullptr, nullptr, 0);
   }
   return cudaGetLastError() == cudaSuccess ? 0 : -8;
 }
@@ -845,14 +857,14 @@ int launch_gather_dq(AttnBwdParams& p, cudaStream_t stream) {
   const int sms = sm_count();
   p.splits = 1;
   const long long items = (long long)p.B * p.H * p.M * column_blocks(p.D);
-  dq<<<(unsigned)(items < sms ? items : sms), kThreadsB, kSmem, stream>>>(p, DenseTileMaps{}, DenseTileMaps{});
+  dq<<<(unsigned)(items < sms ? items : sms), threads_of(kDqGather), kSmem, stream>>>(p, DenseTileMaps{}, DenseTileMaps{});
   return cudaGetLastError() == cudaSuccess ? 0 : -8;
 }
 
 template <bool kFp16>
 int launch_type(AttnBwdParams& p, const Plan& w, bool gather, cudaStream_t stream) {
   // (fp16: at most kMaxBlocks CTAs per head, whose maxima are kept apart)
-  const int bh = p.B * p.H, per = (std::max(p.M * 128, kFp16 ? p.Sk : 0) + 63) / 64;
+  const int bh = p.B * p.H, per = (std::max(p.stat_rows, kFp16 ? p.Sk : 0) + 63) / 64;
   p.max_blocks = std::min(per, kFp16 ? kMaxBlocks : std::max(1, 148 * 8 * 4 / bh));
   attn_bwd_stats_kernel<kFp16><<<dim3((unsigned)p.max_blocks, (unsigned)bh), 256, 0, stream>>>(p);
   if (gather) {
@@ -877,6 +889,7 @@ int64_t attn_bwd_workspace_bytes(const AttnBwdParams& p, bool gather, bool) { re
 
 int launch_attn_bwd(AttnBwdParams& p, bool gather, bool fp16, void* workspace, cudaStream_t stream) {
   const Plan w = make_plan(p, gather);
+  p.stat_rows = w.stat_rows;
   uint8_t* ws = static_cast<uint8_t*>(workspace);
   p.neg_lse2 = reinterpret_cast<float*>(ws);
   p.neg_delta = reinterpret_cast<float*>(ws + w.stats);

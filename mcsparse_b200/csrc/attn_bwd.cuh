@@ -98,6 +98,12 @@ __device__ __forceinline__ uint32_t pack16(float a, float b) {
   else return pack_bf16x2(a, b);
 }
 
+// N consecutive fp32 columns of this thread's lane (N a multiple of 32); complete after tmem_wait_ld
+template <int N>
+__device__ __forceinline__ void load_columns(uint32_t taddr, uint32_t* r) {
+#pragma unroll
+  for (int q = 0; q < N; q += 32) tmem_ld32(taddr + q, *reinterpret_cast<uint32_t(*)[32]>(r + q));
+}
 // two 16-bit values as packed fp32
 template <bool kFp16>
 __device__ __forceinline__ unsigned long long unpack16(uint32_t u) {

@@ -394,7 +394,7 @@ __global__ void __launch_bounds__(kThreadsG, 1) attn_bwd_gather_dkv_kernel(const
                 warp_copy_rows<DB>(s_base + (is_do ? L::kDO : L::kQ), 128, (q & 3) * 32, row_of(it, (q & 3) * 32 + lane), p.D, src, 2 * (size_t)st[1], p.q);
                 if ((q & 3) == 0)
                   cp_async16(s_base + L::kStat + (is_do ? 512 : 0) + lane * 16,
-                             (is_do ? p.neg_delta_kv : p.neg_lse2) + ((size_t)it.bh * p.M + it.m) * 128 + lane * 4);
+                             (is_do ? p.neg_delta_kv : p.neg_lse2) + (size_t)it.bh * p.stat_rows + it.m * 128 + lane * 4);
                 cp_async_arrive_noinc(bar(L::kAFull));
               }
               batch = batch == kLoadWarps - 1 ? 0 : batch + 1;

@@ -185,7 +185,8 @@ struct AttnBwdParams {
   float scale, scale_log2;                    // softmax scale; times log2(e)
   float out_scale;                            // factor of dq and dk: the scale, or 0 where a single key leaves no gradient
   // workspace
-  float *neg_lse2, *neg_delta;                // (B*H, M, 128): -(lse log2 e) (+ kBiasFp16), -rowsum(dout o out); -inf, 0 behind the last row
+  int stat_rows;                              // rows per head of the next three, at least 128 M
+  float *neg_lse2, *neg_delta;                // (B*H, stat_rows): -(lse log2 e) (+ kBiasFp16), -rowsum(dout o out); -inf, 0 behind the last row
   float* neg_delta_kv;                        // neg_delta less the row's sum of dS: what the key side uses (written with dQ)
   float2* row_max;                            // fp16: (B*H, 32) largest norms of rows of dout and of v that each CTA of the statistics saw
   int max_blocks;                             // CTAs per head of the statistics (at most 32)
