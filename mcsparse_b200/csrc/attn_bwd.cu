@@ -161,9 +161,9 @@ struct SmemB {
   static constexpr int kStat = kRingOff + kRing * G::kTileBytes;           // kDkv: TN floats per slot, lse2 with Q, delta with dO; kDq: sums of dS
   static constexpr int kStatBytes = kRing * TN * 4 > 1536 ? kRing * TN * 4 : 1536;
   static constexpr int kBars = kStat + kStatBytes;
-  static constexpr int kFull = 0, kEmpty = kRing, kAFull = 2 * kRing, kAEmpty = kAFull + 1, kSFull = kAEmpty + 1, kSFree = kSFull + 1, kDPFull = kSFree + 1,
-                       kPReady = kDPFull + 1, kDSReady = kPReady + 1, kOFull = kDSReady + 1, kOFree = kOFull + 1, kRowSum = kOFree + 1,
-                       kDrain = kRowSum + 1, kCount = kDrain + 1;
+  static constexpr int kFull = 0, kEmpty = kRing, kAFull = 2 * kRing, kAEmpty = kAFull + 1, kSFull = kAEmpty + 1, kSFree = kSFull + 1,
+                       kDPFull = kSFree + 1, kPReady = kDPFull + 1, kDSReady = kPReady + 1, kOFull = kDSReady + 1, kOFree = kOFull + 1,
+                       kRowSum = kOFree + 1, kDrain = kRowSum + 1, kCount = kDrain + 2;
   static constexpr int kSlot = kBars + kCount * 8;
   static constexpr int kDynamic = kSlot + 16;
   static constexpr uint32_t kColS = 0, kColDP = TN, kColA = 2 * TN, kWidth = DB > 2 ? 192 : DB * 64, kColB = kColA + kWidth;
@@ -172,10 +172,10 @@ template <int DB, int TN>
 constexpr bool fits = SmemB<DB, TN>::kDynamic <= kMaxSmem && SmemB<DB, TN>::kColB + SmemB<DB, TN>::kWidth <= 512;
 static_assert(fits<1, 128> && fits<2, 128> && fits<3, 64> && fits<4, 64>, "227 KB of shared memory, 512 columns of tensor memory");
 
-// Warps: eight softmax warps, the issuer, then for the dense modes the producers of the resident tiles and of the ring, for gathered keys
-// seven warps that copy both: 512 threads of 128 registers.  (24 heads x 256 groups x 2,048 keys x 128: three warps, which leave 168
+// Warps: eight softmax warps, two issuers, then for the dense modes the producers of the resident tiles and of the ring, for gathered keys
+// six warps that copy both: 512 threads of 128 registers.  (24 heads x 256 groups x 2,048 keys x 128: three warps, which leave 168
 // registers, 1.63 ms, four 1.54, seven 1.48.)
-constexpr int kIssueWarp = 8, kLoadWarp0 = 9, kGatherWarps = 7;
+constexpr int kIssueWarp = 8, kScoreWarp = 9, kLoadWarp0 = 10, kGatherWarps = 6;
 constexpr int threads_of(int mode) { return mode == kDqGather ? 32 * (kLoadWarp0 + kGatherWarps) : 384; }
 
 // Blocks of output columns: one, or two of 128 where tensor memory does not hold both sums at full width.
@@ -242,7 +242,7 @@ __global__ void __launch_bounds__(threads_of(kMode), 1) attn_bwd_kernel(const At
   if (tid == 0) {
     for (int i = 0; i < R; ++i) { mbar_init(bar(L::kFull + i), kGather ? TN : 1); mbar_init(bar(L::kEmpty + i), 1); }
     mbar_init(bar(L::kAFull), kGather ? 256 : 1);
-    mbar_init(bar(L::kAEmpty), 1);
+    mbar_init(bar(L::kAEmpty), 2);
     mbar_init(bar(L::kSFull), 1);
     mbar_init(bar(L::kSFree), kSoftmaxWarps);
     mbar_init(bar(L::kDPFull), 1);
@@ -251,7 +251,7 @@ __global__ void __launch_bounds__(threads_of(kMode), 1) attn_bwd_kernel(const At
     mbar_init(bar(L::kOFull), 1);
     mbar_init(bar(L::kOFree), kSoftmaxWarps);
     mbar_init(bar(L::kRowSum), kSoftmaxWarps);
-    mbar_init(bar(L::kDrain), 1);
+    for (int i = 0; i < 2; ++i) mbar_init(bar(L::kDrain + i), 1);
     mbar_fence_init();
   }
   if (warp == kIssueWarp) {
@@ -333,7 +333,7 @@ __global__ void __launch_bounds__(threads_of(kMode), 1) attn_bwd_kernel(const At
         // those are read, dS over the second half
         constexpr int kStep = 32;
         static_assert(kStep >= HC / 2, "P overwrites columns that have been read");
-        uint32_t dp[kStep], pk[HC / 2];
+        uint32_t dp[kStep];
         load_columns<kStep>(tDP, dp);
         tmem_wait_ld();
 #pragma unroll
@@ -343,10 +343,7 @@ __global__ void __launch_bounds__(threads_of(kMode), 1) attn_bwd_kernel(const At
         warp_arrive(bar(L::kPReady));
 #pragma unroll
         for (int s0 = 0; s0 < HC; s0 += kStep) {
-          if (s0 > 0) {
-            load_columns<kStep>(tDP + s0, dp);
-            tmem_wait_ld();
-          }
+          uint32_t pk[kStep / 2];
 #pragma unroll
           for (int d = 0; d < kStep; d += 4) {
             const int e = s0 + d;
@@ -362,18 +359,27 @@ __global__ void __launch_bounds__(threads_of(kMode), 1) attn_bwd_kernel(const At
             d0 = f2_mul(f2_pack(__uint_as_float(sc[e]), __uint_as_float(sc[e + 1])), d0);
             d1 = f2_mul(f2_pack(__uint_as_float(sc[e + 2]), __uint_as_float(sc[e + 3])), d1);
             const float2 y0 = f2_unpack(d0), y1 = f2_unpack(d1);
-            pk[e / 2] = pack16<kFp16>(y0.x, y0.y);
-            pk[e / 2 + 1] = pack16<kFp16>(y1.x, y1.y);
+            pk[d / 2] = pack16<kFp16>(y0.x, y0.y);
+            pk[d / 2 + 1] = pack16<kFp16>(y1.x, y1.y);
             if constexpr (!kRowsAreKeys) {
               es[0] = f2_add(es[0], d0);
               es[1] = f2_add(es[1], d1);
-              rs[0] = f2_add(rs[0], unpack16<kFp16>(pk[e / 2]));
-              rs[1] = f2_add(rs[1], unpack16<kFp16>(pk[e / 2 + 1]));
+              rs[0] = f2_add(rs[0], unpack16<kFp16>(pk[d / 2]));
+              rs[1] = f2_add(rs[1], unpack16<kFp16>(pk[d / 2 + 1]));
             }
           }
-        }
+          // (columns from HC / 2 on: those of the second step have been read, or are not there)
+          if (s0 + kStep < HC) {
+            // ... so the first step's dS waits in registers until the second step's dP has been copied
+            uint32_t next[kStep];
+            load_columns<kStep>(tDP + s0 + kStep, next);
+            tmem_wait_ld();
 #pragma unroll
-        for (int q = 0; q < HC / 16; ++q) tmem_st8(tDP + HC / 2 + q * 8, *reinterpret_cast<const uint32_t(*)[8]>(&pk[q * 8]));
+            for (int i = 0; i < kStep; ++i) dp[i] = next[i];
+          }
+#pragma unroll
+          for (int q = 0; q < kStep / 16; ++q) tmem_st8(tDP + HC / 2 + s0 / 2 + q * 8, *reinterpret_cast<const uint32_t(*)[8]>(&pk[q * 8]));
+        }
         tmem_wait_st();
         tc_fence_before();
         warp_arrive(bar(L::kDSReady));
@@ -466,8 +472,9 @@ __global__ void __launch_bounds__(threads_of(kMode), 1) attn_bwd_kernel(const At
       ++ic;
     }
     tc_fence_before();
-  } else if (warp == kIssueWarp) {
-    // ---- issuer of every product
+  } else if (warp == kIssueWarp || warp == kScoreWarp) {
+    // ---- issuers of the products: S by one warp, dP and the sums, whose order matters, by the other.  A product of eight steps costs the
+    // issuing warp as long as it takes the tensor pipe; one warp for all four had the pipe wait for it.
     constexpr uint32_t kFmt = kFp16 ? 0u : 1u;
     constexpr uint32_t idesc_s = mma_idesc(kFmt, kFmt, 0, 0, 128, TN);
     const bool leader = elect_one();
@@ -483,78 +490,96 @@ __global__ void __launch_bounds__(threads_of(kMode), 1) attn_bwd_kernel(const At
     // accumulated nine times)
     auto scores = [&](uint32_t d, uint32_t a_tile, int load) {
       const uint32_t alo = lo_kmajor(a_tile), blo = lo_kmajor(sRing(load % R));
-#pragma unroll
-      for (int j = 0; j < DB * 4; ++j) {
+      auto step = [&](int j) {
         const uint32_t in = (j & 3) * 2;
-        if (leader && j < kd) mma_f16_ss(d, desc_lo(alo + (j >> 2) * (16384 >> 4) + in), desc_lo(blo + (j >> 2) * (TN * 128 >> 4) + in), idesc_s, j > 0);
+        if (leader) mma_f16_ss(d, desc_lo(alo + (j >> 2) * (16384 >> 4) + in), desc_lo(blo + (j >> 2) * (TN * 128 >> 4) + in), idesc_s, j > 0);
+      };
+      if (kd == DB * 4) {
+#pragma unroll
+        for (int j = 0; j < DB * 4; ++j) step(j);
+      } else {
+#pragma unroll
+        for (int j = 0; j < DB * 4; ++j)
+          if (j < kd) step(j);
       }
     };
-    // sum over a tile of T rows: the operand of half x of the rows lies HC columns behind that of the first half
+    // sum over a tile of T rows; the operands of the two halves of the columns lie HC columns apart
     auto sum = [&](uint32_t d, uint32_t a, int load, const Item& it, uint32_t idesc, bool first) {
       const uint32_t blo = lo_mnmajor(sRing(load % R) + (it.c0 >> 6) * TN * 128, TN * 128);
 #pragma unroll
       for (int j = 0; j < TN / 16; ++j)
-        if (leader) mma_f16_ts(d, a + (j / (TN / 32)) * HC + (j % (TN / 32)) * 8, desc_lo(blo + j * (2048 >> 4)), idesc, !first || j > 0);
+        if (leader) mma_f16_ts(d, a + (j / (HC / 16)) * HC + (j % (HC / 16)) * 8, desc_lo(blo + j * (2048 >> 4)), idesc, !first || j > 0);
     };
-    // S of the tile with running number gs: its scores' columns are free once the tile before has been copied out
-    auto score_tile = [&](int gs) {
-      wait_full(2 * gs);
-      if (ok && gs > 0) ok = mbar_wait(bar(L::kSFree), (gs - 1) & 1, p.status, 143);
-      if (!ok) return;
-      tc_fence_after();
-      scores(tmem + L::kColS, s_base + L::kA0, 2 * gs);
-      if (leader) tc_commit(bar(L::kSFull));
-    };
-    auto dp_tile = [&](int gs, bool last) {
-      wait_full(2 * gs + 1);
-      if (!ok) return;
-      scores(tmem + L::kColDP, s_base + L::kA1, 2 * gs + 1);
-      if (leader) {
-        tc_commit(bar(L::kDPFull));
-        if (!kRowsAreKeys) tc_commit(bar(L::kEmpty + (2 * gs + 1) % R));
-        if (last) tc_commit(bar(L::kAEmpty));
-      }
-    };
-#pragma unroll 1
-    for (int item = blockIdx.x; item < n_items && ok; item += gridDim.x) {
-      const Item it = decode(item);
-      const uint32_t idesc_o = mma_idesc(kFmt, kFmt, 0, 1, 128, it.ncol);
+    auto wait_resident = [&]() {
       ok = mbar_wait(bar(L::kAFull), ic & 1, p.status, 137);
-      if (!ok) break;
+      if (!ok) return;
       if constexpr (kGather) fence_proxy_async_smem();
       tc_fence_after();
-      score_tile(g);
-      if (ok) dp_tile(g, it.t1 - it.t0 == 1);
-      if (ok && it.t1 - it.t0 > 1) score_tile(g + 1);
-      if (!ok) break;
+    };
+    // (tiles of 64 rows, whose products are short, do better in any order: 18,944 x 144 takes 385 us a side against 460)
+    constexpr bool kOrdered = TN == 128;
+    if (warp == kScoreWarp) {
 #pragma unroll 1
-      for (int t = it.t0; t < it.t1; ++t, ++g) {
-        const bool first = t == it.t0, last = t == it.t1 - 1;
-        const int n = 2 * g;
-        ok = mbar_wait(bar(L::kPReady), g & 1, p.status, 138);
-        if (ok && first && ic > 0) ok = mbar_wait(bar(L::kOFree), (ic - 1) & 1, p.status, 139);
-        if (!ok) break;
-        tc_fence_after();
-        sum(tmem + L::kColA, tmem + L::kColDP, kRowsAreKeys ? n + 1 : n, it, idesc_o, first);
-        if (kRowsAreKeys && leader) tc_commit(bar(L::kEmpty + (n + 1) % R));
-        ok = mbar_wait(bar(L::kDSReady), g & 1, p.status, 140);
-        if (!ok) break;
-        tc_fence_after();
-        sum(tmem + L::kColB, tmem + L::kColDP + HC / 2, n, it, idesc_o, first);
-        if (leader) {
-          tc_commit(bar(L::kEmpty + n % R));
-          if (last) tc_commit(bar(L::kOFull));
+      for (int item = blockIdx.x; item < n_items && ok; item += gridDim.x, ++ic) {
+        const Item it = decode(item);
+        wait_resident();
+#pragma unroll 1
+        for (int t = it.t0; t < it.t1 && ok; ++t, ++g) {
+          // Its columns are free once the tile before has been copied out.  That tile's dP goes first: the softmax waits for it longer.
+          // (dP of tile g in turn is issued behind a wait for this product, so neither barrier can run two phases ahead of its waits.)
+          wait_full(2 * g);
+          if (ok && kOrdered && t > it.t0) ok = mbar_wait(bar(L::kDPFull), (g - 1) & 1, p.status, 144);
+          if (ok && g > 0) ok = mbar_wait(bar(L::kSFree), (g - 1) & 1, p.status, 143);
+          if (!ok) break;
+          tc_fence_after();
+          scores(tmem + L::kColS, s_base + L::kA0, 2 * g);
+          if (leader) {
+            tc_commit(bar(L::kSFull));
+            if (t == it.t1 - 1) tc_commit(bar(L::kAEmpty));
+          }
         }
-        if (!last) dp_tile(g + 1, t + 2 == it.t1);
-        if (ok && t + 2 < it.t1) score_tile(g + 2);
-        if (!ok) break;
       }
-      ++ic;
+    } else {
+#pragma unroll 1
+      for (int item = blockIdx.x; item < n_items && ok; item += gridDim.x, ++ic) {
+        const Item it = decode(item);
+        const uint32_t idesc_o = mma_idesc(kFmt, kFmt, 0, 1, 128, it.ncol);
+        wait_resident();
+        if (!ok) break;
+#pragma unroll 1
+        for (int t = it.t0; t < it.t1; ++t, ++g) {
+          const bool first = t == it.t0, last = t == it.t1 - 1;
+          const int n = 2 * g;
+          if (kOrdered && !first) ok = mbar_wait(bar(L::kSFull), g & 1, p.status, 145);
+          wait_full(n + 1);
+          if (!ok) break;
+          scores(tmem + L::kColDP, s_base + L::kA1, n + 1);
+          if (leader) {
+            tc_commit(bar(L::kDPFull));
+            if (!kRowsAreKeys) tc_commit(bar(L::kEmpty + (n + 1) % R));
+            if (last) tc_commit(bar(L::kAEmpty));
+          }
+          ok = mbar_wait(bar(L::kPReady), g & 1, p.status, 138);
+          if (ok && first && ic > 0) ok = mbar_wait(bar(L::kOFree), (ic - 1) & 1, p.status, 139);
+          if (!ok) break;
+          tc_fence_after();
+          sum(tmem + L::kColA, tmem + L::kColDP, kRowsAreKeys ? n + 1 : n, it, idesc_o, first);
+          if (kRowsAreKeys && leader) tc_commit(bar(L::kEmpty + (n + 1) % R));
+          ok = mbar_wait(bar(L::kDSReady), g & 1, p.status, 140);
+          if (!ok) break;
+          tc_fence_after();
+          sum(tmem + L::kColB, tmem + L::kColDP + HC / 2, n, it, idesc_o, first);
+          if (leader) {
+            tc_commit(bar(L::kEmpty + n % R));
+            if (last) tc_commit(bar(L::kOFull));
+          }
+        }
+      }
     }
     if (!ok) {
       // error path: let outstanding products retire before tensor memory is released
-      if (leader) tc_commit(bar(L::kDrain));
-      mbar_wait_quiet(bar(L::kDrain), 0, 1 << 20);
+      if (leader) tc_commit(bar(L::kDrain + (warp == kScoreWarp ? 1 : 0)));
+      mbar_wait_quiet(bar(L::kDrain + (warp == kScoreWarp ? 1 : 0)), 0, 1 << 20);
     }
     __syncwarp();
     tc_fence_before();
