@@ -301,43 +301,30 @@ __global__ void __launch_bounds__(kThreadsG, 1) attn_bwd_gather_dkv_kernel(const
       if (!ok) break;
       fence_proxy_async_smem();
       tc_fence_after();
-      scores(tmem + kColS, s_base + L::kQ, bar(L::kSFull));
-      if (ok) scores(tmem + kColDP, s_base + L::kDO, bar(L::kDPFull));
 #pragma unroll 1
       for (int t = 0; t < it.T && ok; ++t, ++g) {
-        ok = mbar_wait(bar(L::kPReady), g & 1, p.status, 156);
-        if (ok && blk > 0) ok = mbar_wait(bar(L::kOFree), (blk - 1) & 1, p.status, 157);
-        if (!ok) break;
-        tc_fence_after();
-        out_product(tmem + kColDV, tmem + kColS, s_base + L::kDO, 0);
-        if (leader) tc_commit(bar(L::kOFull));
-        ok = mbar_wait(bar(L::kDSReady), g & 1, p.status, 158);
-        if (ok && blk > 0) ok = mbar_wait(bar(L::kOFree + 1), (blk - 1) & 1, p.status, 162);
-        if (!ok) break;
-        tc_fence_after();
-        out_product(tmem + kColDK, tmem + kColDP, s_base + L::kQ, 0);
-        if (leader) tc_commit(bar(L::kOFull + 1));
-        ++blk;
 #pragma unroll 1
-        for (int cb = 1; cb < CB; ++cb, ++blk) {
-          ok = mbar_wait(bar(L::kOFree), (blk - 1) & 1, p.status, 159);
+        for (int i = 0; i < 2 && ok; ++i)
+          scores(tmem + (i == 0 ? kColS : kColDP), s_base + (i == 0 ? L::kQ : L::kDO), bar(i == 0 ? L::kSFull : L::kDPFull));
+        if (!ok) break;
+        ok = mbar_wait(bar(L::kPReady), g & 1, p.status, 156);
+        if (!ok) break;
+#pragma unroll 1
+        for (int cb = 0; cb < CB; ++cb, ++blk) {
+          if (blk > 0) ok = mbar_wait(bar(L::kOFree), (blk - 1) & 1, p.status, 157);
           if (!ok) break;
           tc_fence_after();
           out_product(tmem + kColDV, tmem + kColS, s_base + L::kDO, cb);
           if (leader) tc_commit(bar(L::kOFull));
-          ok = mbar_wait(bar(L::kOFree + 1), (blk - 1) & 1, p.status, 162);
+          if (cb == 0) ok = mbar_wait(bar(L::kDSReady), g & 1, p.status, 158);
+          if (ok && blk > 0) ok = mbar_wait(bar(L::kOFree + 1), (blk - 1) & 1, p.status, 162);
           if (!ok) break;
           tc_fence_after();
           out_product(tmem + kColDK, tmem + kColDP, s_base + L::kQ, cb);
           if (leader) tc_commit(bar(L::kOFull + 1));
         }
         if (!ok) break;
-        if (t + 1 < it.T) {
-          scores(tmem + kColS, s_base + L::kQ, bar(L::kSFull));
-          if (ok) scores(tmem + kColDP, s_base + L::kDO, bar(L::kDPFull));
-        } else if (leader) {
-          tc_commit(bar(L::kAEmpty));
-        }
+        if (t == it.T - 1 && leader) tc_commit(bar(L::kAEmpty));
       }
     }
     if (!ok) {
