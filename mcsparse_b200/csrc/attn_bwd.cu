@@ -280,7 +280,9 @@ __global__ void __launch_bounds__(threads_of(kMode), 1) attn_bwd_kernel(const At
       const Item it = decode(item);
       const float c = ds_scale<kFp16>(p, it.bh);
       const unsigned long long c2 = f2_pack(c, c);
-      unsigned long long nl2 = 0, nd2 = 0, rs[2] = {0, 0}, es[2] = {0, 0};   // kDq: this row's statistics, sums of its dS rounded and not
+      unsigned long long nl2 = 0, nd2 = 0, es[2] = {0, 0};
+      float rs[4] = {0.f, 0.f, 0.f, 0.f};
+        // kDq: this row's statistics, sums of its dS rounded and not
       if constexpr (!kRowsAreKeys) {
         const size_t si = (size_t)it.bh * p.stat_rows + it.m * 128 + r_in;
         const float nl = p.neg_lse2[si], ndl = p.neg_delta[si];
@@ -364,8 +366,8 @@ __global__ void __launch_bounds__(threads_of(kMode), 1) attn_bwd_kernel(const At
             if constexpr (!kRowsAreKeys) {
               es[0] = f2_add(es[0], d0);
               es[1] = f2_add(es[1], d1);
-              rs[0] = f2_add(rs[0], unpack16<kFp16>(pk[d / 2]));
-              rs[1] = f2_add(rs[1], unpack16<kFp16>(pk[d / 2 + 1]));
+              add_pair<kFp16>(pk[d / 2], rs[0], rs[1]);
+              add_pair<kFp16>(pk[d / 2 + 1], rs[2], rs[3]);
             }
           }
           // (columns from HC / 2 on: those of the second step have been read, or are not there)
@@ -390,8 +392,8 @@ __global__ void __launch_bounds__(threads_of(kMode), 1) attn_bwd_kernel(const At
       if constexpr (!kRowsAreKeys) {
         // the row's sums of dS from its two threads; the other's are read before this item's kOFree, so before they are written again
         float* sums = reinterpret_cast<float*>(smem + L::kStat);
-        const float2 a = f2_unpack(rs[0]), b = f2_unpack(rs[1]), a2 = f2_unpack(es[0]), b2 = f2_unpack(es[1]);
-        sums[x * 128 + r_in] = (a.x + a.y) + (b.x + b.y);
+        const float2 a2 = f2_unpack(es[0]), b2 = f2_unpack(es[1]);
+        sums[x * 128 + r_in] = (rs[0] + rs[1]) + (rs[2] + rs[3]);
         off = (a2.x + a2.y) + (b2.x + b2.y);
         if (x == 1) sums[256 + r_in] = off;
         warp_arrive(bar(L::kRowSum));
@@ -799,7 +801,7 @@ Plan make_plan(const AttnBwdParams& p, bool gather) {
   if (gather) {
     w.dq_splits = w.kv_splits = 1;
   } else {
-    const double tile_us = p.D <= 64 ? 1.5 : (p.D <= 128 ? 1.9 : 1.5);
+    const double tile_us = p.D <= 64 ? 1.3 : (p.D <= 128 ? 1.6 : 1.2);
     w.dq_splits = pick_splits(bh * p.M * blocks, (p.Sk + TN - 1) / TN, tile_us, (double)bh * p.Sq * (2 * p.D + 8) * 4);
     w.kv_splits = pick_splits(bh * ((p.Sk + 127) / 128) * blocks, (p.Sq + TN - 1) / TN, tile_us, (double)bh * p.Sk * 2 * p.D * 4);
   }

@@ -104,15 +104,13 @@ __device__ __forceinline__ void load_columns(uint32_t taddr, uint32_t* r) {
 #pragma unroll
   for (int q = 0; q < N; q += 32) tmem_ld32(taddr + q, *reinterpret_cast<uint32_t(*)[32]>(r + q));
 }
-// two 16-bit values as packed fp32
+// lo += the lower, hi += the upper of two 16-bit values: fp32 additions that take the 16-bit operand as it is
 template <bool kFp16>
-__device__ __forceinline__ unsigned long long unpack16(uint32_t u) {
-  if constexpr (kFp16) {
-    const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&u));
-    return f2_pack(f.x, f.y);
-  } else {
-    return f2_pack(bf16_lo(u), bf16_hi(u));
-  }
+__device__ __forceinline__ void add_pair(uint32_t u, float& lo, float& hi) {
+  if constexpr (kFp16)
+    asm("{\n\t.reg .b16 l, h;\n\tmov.b32 {l, h}, %2;\n\tadd.rn.f32.f16 %0, l, %0;\n\tadd.rn.f32.f16 %1, h, %1;\n\t}\n" : "+f"(lo), "+f"(hi) : "r"(u));
+  else
+    asm("{\n\t.reg .b16 l, h;\n\tmov.b32 {l, h}, %2;\n\tadd.rn.f32.bf16 %0, l, %0;\n\tadd.rn.f32.bf16 %1, h, %1;\n\t}\n" : "+f"(lo), "+f"(hi) : "r"(u));
 }
 // sixteen fp32 values, rounded, into eight tensor-memory columns of this thread's lane
 template <bool kFp16>

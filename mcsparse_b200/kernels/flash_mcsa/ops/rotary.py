@@ -179,6 +179,9 @@ class RotaryEmbedding:
         else:
             with torch.cuda.device(device):
                 _lib.launch("mcs_rotary", a, device, "mcs_rotary")
+        if inplace:
+            for t in tensors:
+                torch.autograd.graph.increment_version(t)      # what autograd saved of it is no longer there
         return outs
 
     def rotate(self, *tensors: Tensor, positions: Tensor, inplace: bool = False):
