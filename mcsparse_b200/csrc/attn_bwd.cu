@@ -48,7 +48,10 @@ __global__ void __launch_bounds__(256) attn_bwd_stats_kernel(const AttnBwdParams
   const uint8_t* gb = reinterpret_cast<const uint8_t*>(p.dout) + 2 * ((size_t)b * p.dout_stride[0] + (size_t)h * p.dout_stride[2]);
   const uint8_t* ob = reinterpret_cast<const uint8_t*>(p.out) + 2 * ((size_t)b * p.out_stride[0] + (size_t)h * p.out_stride[2]);
   float m_do = 0.f, m_v = 0.f;
-  for (int base = blockIdx.x * (16 * kRows); base < rows; base += gridDim.x * (16 * kRows)) {
+  // fp16: every second CTA takes rows of v instead
+  const int share = kFp16 ? 2 : 1, blk = blockIdx.x / share, step = gridDim.x / share;
+  const bool of_v = kFp16 && blockIdx.x % 2 == 1;
+  for (int base = blk * (16 * kRows); base < rows && !of_v; base += step * (16 * kRows)) {
     int row[kRows];
     float dot[kRows] = {}, sq[kRows] = {};
 #pragma unroll
@@ -97,7 +100,7 @@ __global__ void __launch_bounds__(256) attn_bwd_stats_kernel(const AttnBwdParams
   }
   if constexpr (kFp16) {
     const uint8_t* vb = reinterpret_cast<const uint8_t*>(p.v) + 2 * ((size_t)b * p.v_stride[0] + (size_t)h * p.v_stride[2]);
-    for (int base = blockIdx.x * (16 * kRows); base < p.Sk; base += gridDim.x * (16 * kRows)) {
+    for (int base = blk * (16 * kRows); base < p.Sk && of_v; base += step * (16 * kRows)) {
       float sq[kRows] = {};
       for (int c = l16; c < chunks; c += 16) {
         uint4 x[kRows];
@@ -892,7 +895,7 @@ template <bool kFp16>
 int launch_type(AttnBwdParams& p, const Plan& w, bool gather, cudaStream_t stream) {
   // (fp16: at most kMaxBlocks CTAs per head, whose maxima are kept apart)
   const int bh = p.B * p.H, per = (std::max(p.stat_rows, kFp16 ? p.Sk : 0) + 63) / 64;
-  p.max_blocks = std::min(per, kFp16 ? kMaxBlocks : std::max(1, 148 * 8 * 4 / bh));
+  p.max_blocks = kFp16 ? 2 * std::min(per, kMaxBlocks / 2) : std::min(per, std::max(1, 148 * 8 * 4 / bh));
   attn_bwd_stats_kernel<kFp16><<<dim3((unsigned)p.max_blocks, (unsigned)bh), 256, 0, stream>>>(p);
   if (gather) {
     const int db = padded_blocks(p.D);

@@ -24,13 +24,17 @@ constexpr float kBiasFp16 = 14.f;
 constexpr int kSoftmaxWarps = 8;       // warps 0-3 take the first half of a score tile's columns, 4-7 the second; lane == row
 
 // Power of two by which dS / 2^14 may be multiplied (see above), from the largest row norms; 1 for bf16.  A whole warp calls it.
-constexpr int kMaxBlocks = 32;          // CTAs per head of the statistics, each of which leaves its own maxima
+constexpr int kMaxBlocks = 64;          // CTAs per head of the statistics, each of which leaves its own maxima
 template <bool kFp16>
 __device__ __forceinline__ float ds_scale(const AttnBwdParams& p, int bh) {
   if constexpr (!kFp16) return 1.f;
   const int lane = threadIdx.x & 31;
   const float2* parts = p.row_max + (size_t)bh * kMaxBlocks;
-  float2 v = lane < p.max_blocks ? parts[lane] : make_float2(0.f, 0.f);
+  float2 v = make_float2(0.f, 0.f);
+  for (int i = lane; i < p.max_blocks; i += 32) {
+    const float2 m = parts[i];
+    v = make_float2(fmaxf(v.x, m.x), fmaxf(v.y, m.y));
+  }
 #pragma unroll
   for (int off = 16; off >= 1; off >>= 1) {
     v.x = fmaxf(v.x, __shfl_xor_sync(0xffffffffu, v.x, off));

@@ -476,32 +476,26 @@ constexpr int kManyEntries = 64;
 
 template <int C>   // float4 columns per lane
 __device__ __forceinline__ void add_rows(const float4* src, int n, int lane, int cols4, float4 (&acc)[C]) {
-  constexpr int kUnroll = 4;
-  int i = 0;
-  for (; i + kUnroll <= n; i += kUnroll) {
+  constexpr int kUnroll = C == 1 ? 8 : (C == 2 ? 4 : 2);
+#pragma unroll 1
+  for (int i = 0; i < n; i += kUnroll, src += (size_t)kUnroll * cols4) {
     float4 v[kUnroll][C];
 #pragma unroll
     for (int u = 0; u < kUnroll; ++u)
 #pragma unroll
-      for (int q = 0; q < C; ++q)
-        if (lane + q * 32 < cols4) v[u][q] = __ldcs(src + (size_t)(i + u) * cols4 + lane + q * 32);
+      for (int q = 0; q < C; ++q) {
+        v[u][q] = make_float4(0.f, 0.f, 0.f, 0.f);
+        if (i + u < n && lane + q * 32 < cols4) v[u][q] = __ldcs(src + u * cols4 + lane + q * 32);
+      }
 #pragma unroll
     for (int u = 0; u < kUnroll; ++u)
 #pragma unroll
-      for (int q = 0; q < C; ++q)
-        if (lane + q * 32 < cols4) { acc[q].x += v[u][q].x; acc[q].y += v[u][q].y; acc[q].z += v[u][q].z; acc[q].w += v[u][q].w; }
+      for (int q = 0; q < C; ++q) { acc[q].x += v[u][q].x; acc[q].y += v[u][q].y; acc[q].z += v[u][q].z; acc[q].w += v[u][q].w; }
   }
-  for (; i < n; ++i)
-#pragma unroll
-    for (int q = 0; q < C; ++q)
-      if (lane + q * 32 < cols4) {
-        const float4 v = __ldcs(src + (size_t)i * cols4 + lane + q * 32);
-        acc[q].x += v.x; acc[q].y += v.y; acc[q].z += v.z; acc[q].w += v.w;
-      }
 }
 
 template <int C, bool kFp16>
-__global__ void __launch_bounds__(256) attn_bwd_key_sum_kernel(const AttnBwdParams p) {
+__global__ void __launch_bounds__(256, 4) attn_bwd_key_sum_kernel(const AttnBwdParams p) {
   __shared__ float4 part[8][C * 32];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int bh = p.bh0 + blockIdx.y, b = bh / p.H, h = bh % p.H;
@@ -524,18 +518,24 @@ __global__ void __launch_bounds__(256) attn_bwd_key_sum_kernel(const AttnBwdPara
     const int key = key0 + warp;
     int at = 0, n = 0;
     if (key < p.Sk) { at = start[key]; n = start[key + 1] - at; }
-    if (key < p.Sk && n <= kManyEntries) {
+    // first every warp's own key, then the keys of this CTA that have many entries, one after the other
+#pragma unroll 1
+    for (int i = -1; i < 8 && key0 + i < p.Sk; ++i) {
+      int r0 = at, m = n <= kManyEntries ? n : 0;
+      if (i >= 0) {
+        const int a = start[key0 + i], all = start[key0 + i + 1] - a;
+        if (all <= kManyEntries) continue;                   // (uniform over the CTA)
+        r0 = (int)((long long)all * warp / 8);
+        m = (int)((long long)all * (warp + 1) / 8) - r0;
+        r0 += a;
+      }
       float4 acc[C] = {};
-      add_rows<C>(rows + (size_t)at * cols4, n, lane, cols4, acc);
-      store(key, acc);
-    }
-    if (!__syncthreads_or(n > kManyEntries)) continue;
-    for (int i = 0; i < 8 && key0 + i < p.Sk; ++i) {
-      const int a = start[key0 + i], m = start[key0 + i + 1] - a;
-      if (m <= kManyEntries) continue;                       // (uniform over the CTA)
-      const int r0 = (int)((long long)m * warp / 8), r1 = (int)((long long)m * (warp + 1) / 8);
-      float4 acc[C] = {};
-      add_rows<C>(rows + (size_t)(a + r0) * cols4, r1 - r0, lane, cols4, acc);
+      add_rows<C>(rows + (size_t)r0 * cols4, m, lane, cols4, acc);
+      if (i < 0) {
+        if (key < p.Sk && n <= kManyEntries) store(key, acc);
+        if (!__syncthreads_or(n > kManyEntries)) break;
+        continue;
+      }
 #pragma unroll
       for (int q = 0; q < C; ++q) part[warp][lane + q * 32] = acc[q];
       __syncthreads();

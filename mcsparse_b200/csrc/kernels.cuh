@@ -188,8 +188,8 @@ struct AttnBwdParams {
   int stat_rows;                              // rows per head of the next three, at least 128 M
   float *neg_lse2, *neg_delta;                // (B*H, stat_rows): -(lse log2 e) (+ kBiasFp16), -rowsum(dout o out); -inf, 0 behind the last row
   float* neg_delta_kv;                        // neg_delta less the row's sum of dS: what the key side uses (written with dQ)
-  float2* row_max;                            // fp16: (B*H, 32) largest norms of rows of dout and of v that each CTA of the statistics saw
-  int max_blocks;                             // CTAs per head of the statistics (at most 32)
+  float2* row_max;                            // fp16: (B*H, 64) largest norms of rows of dout and of v that each CTA of the statistics saw
+  int max_blocks;                             // CTAs per head of the statistics (fp16: at most 64)
   float* parts;                               // split launches: partial sums
   int splits;
   // gather: entries that name key j of head bh lie at rows [key_start[bh][j], key_start[bh][j + 1]) of that head's block of partial

@@ -86,8 +86,8 @@ def test_entry_point_refusals():
 
 def test_workspace_sizes():
     lib = _lib.lib()
-    # the DiT layer: enough tiles for every SM, so only the rows' statistics (3 floats per row, 32 pairs of maxima per head)
-    assert lib.mcs_dense_attn_bwd_workspace_bytes(raw(Sq=32760, Sk=32760, H=24, D=128)) == 24 * (3 * 32768 * 4 + 32 * 8)
+    # the DiT layer: enough tiles for every SM, so only the rows' statistics (3 floats per row, 64 pairs of maxima per head)
+    assert lib.mcs_dense_attn_bwd_workspace_bytes(raw(Sq=32760, Sk=32760, H=24, D=128)) == 24 * (3 * 32768 * 4 + 64 * 8)
     # few keys, many queries: partial sums of the split queries on top
     assert lib.mcs_dense_attn_bwd_workspace_bytes(raw(Sq=32760, Sk=512, H=1, D=128)) > 4 * 2 * 512 * 2 * 128
     # gather: the contributions of as many heads at a time as fit 4 GiB, at least one head's
