@@ -142,10 +142,20 @@ __global__ void __launch_bounds__(256) attn_bwd_stats_kernel(const AttnBwdParams
 //   kDkv             K    V    Q    dO     rows: keys (S^T, dP^T)          dV += P^T dO  dK += dS^T Q
 // Scores lie with the resident row as the tensor-memory lane, so that P and dS are the first operands of the sums where they
 // are.  A softmax thread copies its scores to registers, which frees S for the next tile at once, and computes P there; when dP(t) is
-// complete it reads it and stores P and dS, 16 bits each, over it.  Issue order: sum of P(t), sum of dS(t), dP(t+1), S(t+2).  Products of
-// one thread execute in order, so dP(t+1) may follow the sums that read P(t) and dS(t) without a wait.  The exponentials of t+1 run
-// under the sum of dS(t) and dP(t+1); what the tensor pipe could wait for, dP(t) -> P stored, is covered by S(t+1).  (With P stored over
-// its scores, S(t+1) had to follow the sum of P(t), and the exponentials of t+1 that: @@OLD@@)
+// complete it reads it and stores P and dS, 16 bits each, over it.  One warp issues dP(t), sum of P(t), sum of dS(t), dP(t+1), ...:
+// products of one thread execute in order, so dP(t+1) may follow the sums that read P(t) and dS(t) without a wait.  Another issues
+// S(t+1) behind dP(t).  So the exponentials of t+1 run under the sum of dS(t) and dP(t+1), and S(t+1) covers what the tensor pipe
+// could wait for, dP(t) -> P stored.
+//
+// What bounds it.  Per pair of tiles (128 x 128 x 128) the tensor pipe needs 2,048 cycles, shared memory the same (1,536 for operands
+// at 128 bytes a cycle, 512 for the next tiles), the special-function unit 1,024, and the chain dP -> registers -> dS -> sum of dS -> next dP
+// about 2,400.  One wave of 148 x 148 tiles of one head: 1.61 us a tile on the key side, 1.64 on the query side (about 3,000
+// cycles); D = 64: 1.30 and 1.34; D = 144: 2.35 and 2.45 per 128 rows.  In a loop of calls at 24 heads x 32,760 x 128 the power limit
+// lowers the clock: 39.8 ms for 52.8 TFLOP of products (1.33 PFLOP/s, against 1.41 that the library's largest products sustain).
+// Steps, same call: P stored over its scores, so that S(t+1) had to follow the sum of P(t): 45.6 ms; scores copied out first: 43.5; two issuing
+// warps, and every product issued from one place of the program (with a copy of the issuing code in front of the loop, a tile took 10% to
+// 30% longer), 16-bit dS summed by mixed-precision additions: 39.8.  Measured and not kept: two tiles of 64 rows in flight, one for each half of
+// the softmax warps (D = 64: 1.56 us against 1.44 then); the sum of dS started at half of a tile (1.68 against 1.65).
 //
 // PK: the rows of dS sum to zero, but those of its rounded form, with a delta from a rounded out, do not: they sum to r, and
 // dQ is off by r times the keys that a row looks at, which does not average out where these keys resemble one another (with
@@ -478,8 +488,8 @@ __global__ void __launch_bounds__(threads_of(kMode), 1) attn_bwd_kernel(const At
     }
     tc_fence_before();
   } else if (warp == kIssueWarp || warp == kScoreWarp) {
-    // ---- issuers of the products: S by one warp, dP and the sums, whose order matters, by the other.  A product of eight steps costs the
-    // issuing warp as long as it takes the tensor pipe; one warp for all four had the pipe wait for it.
+    // ---- issuers of the products: S by one warp, dP and the sums, whose order matters, by the other.  Issuing a product's eight steps takes
+    // a warp about as long as they take the tensor pipe; one warp for all four had the pipe wait for it.
     constexpr uint32_t kFmt = kFp16 ? 0u : 1u;
     constexpr uint32_t idesc_s = mma_idesc(kFmt, kFmt, 0, 0, 128, TN);
     const bool leader = elect_one();

@@ -7,8 +7,13 @@
 // order, and the sums (and their bits) do not depend on which CTA came first.  (Adding with atomics in place would move the same bytes
 // through L2 and leave the order to chance.)  Equal entries inside one group have equal contributions, so their order does not matter.
 //
-// Bound: the buffer is written and read once, 8 D bytes each per entry (12.9 GB + 12.9 GB at 24 heads x 256 groups x 2,048 keys x
-// 128), against 5 x 2 x 128 x D operations: memory, by a factor of about three.
+// Bound: the buffer is written and read once, 8 D bytes per entry either way (12.9 GB + 12.9 GB at 24 heads x 256 groups x 2,048
+// keys x 128: 3.9 ms at the copy rate), against 10 x 128 x D operations (1.25 ms): memory.  Measured there: 2.99 ms for the
+// contributions (4.3 TB/s of rows scattered by key; the copy out of tensor memory, through shared memory and the SM's store path,
+// is the longest stage of a tile: 1.6 ms without it), 1.98 ms for the sums (6.5 TB/s, the copy rate).  Steps: every thread storing its own row 4.83 ms; 128
+// contiguous bytes at a time through shared memory 4.44; by warps of their own, under the next tile's P and dS, 3.26; dV released
+// before dK 2.99.  Measured and not kept: rows in the order of groups, contiguous for a tile, gathered by the sums instead: 3.79 ms
+// (against 4.44 then) for the contributions, but 4.53 ms for the sums; dV copied by the softmax warps: 3.21.
 #include "attn_bwd.cuh"
 
 namespace mcs {
@@ -112,7 +117,7 @@ __global__ void __launch_bounds__(1024) attn_bwd_rows_kernel(const AttnBwdParams
 // blocks of up to 128 columns.  Per tile:
 //     S^T = K Q^T, dP^T = V dO^T (rows: gathered keys)  ->  P^T, dS^T in tensor memory, over their scores
 //     dV = P^T dO, dK = dS^T Q, up to 128 columns at a time, copied to the entries' rows by four warps of their own
-// The copy is the longest part of a tile (128 D x 8 bytes through the SM's store path); the next tile's P and dS are computed under it.
+// The copy is the longest part of a tile; the next tile's P and dS are computed under it.
 template <int DB>
 struct SmemG {
   static constexpr int kResBytes = DB * 16384;

@@ -13,7 +13,9 @@
 // Products and sums are 32-bit, with one rounding to the tensors' type.
 //
 // Memory-bound: each element is read once and written once.  A thread owns 16 bytes of a row (half layout: 16 bytes of either
-// half) of one token and walks over heads, so that the angles of its pairs are computed once for all its heads.
+// half) of one token and walks over up to sixteen heads with eight loads in flight, so that the angles of its pairs are computed once for
+// them.  q and k of 24 heads x 32,760 x 128 bf16: 0.128 ms, 6.3 TB/s, 0.96 of the copy rate (0.255 with guarded loads and 64-bit index
+// arithmetic per head).  fp32, 2 x 4,095 x 20 heads x 144, 96 of them rotated: 41 us, 4.6 TB/s (part of it out of L2).
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
