@@ -22,7 +22,9 @@ constexpr int kMaxSmem = 232448;
 
 // ------------------------------------------------------------------------------------------------ row statistics
 // Sixteen lanes per row, four rows at a time: neg_delta = -sum(dout * out) and neg_lse2 of every tile row (memory-bound: dout and out
-// are read once, eight 16-byte loads of a thread in flight), and for fp16 the largest norms of rows of dout and of v.
+// are read once, eight 16-byte loads of a thread in flight), and for fp16 the largest norms of rows of dout and of v.  Only rows that take
+// part in finite results count for these: rows with an infinity or NaN give no finite dS whatever its scale, and rows of v that no group
+// selected (key_start, gathered keys only) may hold anything.
 template <bool kFp16>
 __device__ __forceinline__ float dot8(uint4 a, uint4 b, float acc) {
   const uint32_t x[4] = {a.x, a.y, a.z, a.w}, y[4] = {b.x, b.y, b.z, b.w};
@@ -83,7 +85,7 @@ __global__ void __launch_bounds__(256) attn_bwd_stats_kernel(const AttnBwdParams
         dot[u] += __shfl_xor_sync(0xffffffffu, dot[u], off);
         if constexpr (kFp16) sq[u] += __shfl_xor_sync(0xffffffffu, sq[u], off);
       }
-      m_do = fmaxf(m_do, sq[u]);
+      m_do = fmaxf(m_do, sq[u] < INFINITY ? sq[u] : 0.f);
       const int i = base + u * 16 + sub;
       if (l16 == 0 && i < rows) {
         float nl = -INFINITY;                                // rows behind the last one: P = 0
@@ -100,6 +102,7 @@ __global__ void __launch_bounds__(256) attn_bwd_stats_kernel(const AttnBwdParams
   }
   if constexpr (kFp16) {
     const uint8_t* vb = reinterpret_cast<const uint8_t*>(p.v) + 2 * ((size_t)b * p.v_stride[0] + (size_t)h * p.v_stride[2]);
+    const int32_t* start = p.key_start != nullptr ? p.key_start + (size_t)bh * (p.Sk + 1) : nullptr;
     for (int base = blk * (16 * kRows); base < p.Sk && of_v; base += step * (16 * kRows)) {
       float sq[kRows] = {};
       for (int c = l16; c < chunks; c += 16) {
@@ -107,7 +110,8 @@ __global__ void __launch_bounds__(256) attn_bwd_stats_kernel(const AttnBwdParams
 #pragma unroll
         for (int u = 0; u < kRows; ++u) {
           const int i = base + u * 16 + sub;
-          x[u] = i < p.Sk ? *reinterpret_cast<const uint4*>(vb + 2 * (size_t)i * p.v_stride[1] + c * 16) : make_uint4(0, 0, 0, 0);
+          x[u] = i < p.Sk && (start == nullptr || start[i + 1] > start[i]) ? *reinterpret_cast<const uint4*>(vb + 2 * (size_t)i * p.v_stride[1] + c * 16)
+                                                                           : make_uint4(0, 0, 0, 0);
         }
 #pragma unroll
         for (int u = 0; u < kRows; ++u) sq[u] = dot8<kFp16>(x[u], x[u], sq[u]);
@@ -116,7 +120,7 @@ __global__ void __launch_bounds__(256) attn_bwd_stats_kernel(const AttnBwdParams
       for (int u = 0; u < kRows; ++u) {
 #pragma unroll
         for (int off = 8; off >= 1; off >>= 1) sq[u] += __shfl_xor_sync(0xffffffffu, sq[u], off);
-        m_v = fmaxf(m_v, sq[u]);
+        m_v = fmaxf(m_v, sq[u] < INFINITY ? sq[u] : 0.f);
       }
     }
     __shared__ float2 red[8];
@@ -906,6 +910,11 @@ int launch_type(AttnBwdParams& p, const Plan& w, bool gather, cudaStream_t strea
   // (fp16: at most kMaxBlocks CTAs per head, whose maxima are kept apart)
   const int bh = p.B * p.H, per = (std::max(p.stat_rows, kFp16 ? p.Sk : 0) + 63) / 64;
   p.max_blocks = kFp16 ? 2 * std::min(per, kMaxBlocks / 2) : std::min(per, std::max(1, 148 * 8 * 4 / bh));
+  // (before the statistics, which ask which keys have entries)
+  if (gather) {
+    const int rc = launch_attn_bwd_gather_rows(p, w.segs, stream);
+    if (rc != 0) return rc;
+  }
   attn_bwd_stats_kernel<kFp16><<<dim3((unsigned)p.max_blocks, (unsigned)bh), 256, 0, stream>>>(p);
   if (gather) {
     const int db = padded_blocks(p.D);
@@ -913,7 +922,7 @@ int launch_type(AttnBwdParams& p, const Plan& w, bool gather, cudaStream_t strea
                    : db == 2 ? launch_gather_dq<2, 128, kFp16>(p, stream)
                    : db == 3 ? launch_gather_dq<3, 64, kFp16>(p, stream)
                              : launch_gather_dq<4, 64, kFp16>(p, stream);
-    return rc != 0 ? rc : launch_attn_bwd_gather_dkv(p, kFp16, w.segs, w.heads_per_pass, stream);
+    return rc != 0 ? rc : launch_attn_bwd_gather_dkv(p, kFp16, w.heads_per_pass, stream);
   }
   switch (padded_blocks(p.D)) {
     case 1: return launch_dense<1, 128, kFp16>(p, w, stream);
@@ -937,7 +946,7 @@ int launch_attn_bwd(AttnBwdParams& p, bool gather, bool fp16, void* workspace, c
   p.row_max = reinterpret_cast<float2*>(ws + 3 * w.stats);
   ws += 3 * w.stats + w.row_max;
   p.entry_row = reinterpret_cast<int32_t*>(ws);
-  p.key_start = reinterpret_cast<int32_t*>(ws + w.entries);
+  p.key_start = gather ? reinterpret_cast<int32_t*>(ws + w.entries) : nullptr;
   p.seg_count = reinterpret_cast<int32_t*>(ws + w.entries + w.starts);
   p.block_sum = reinterpret_cast<int32_t*>(ws + w.entries + w.starts + w.counts);
   p.parts = reinterpret_cast<float*>(ws + w.entries + w.starts + w.counts + w.blocks);

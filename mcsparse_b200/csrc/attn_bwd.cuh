@@ -9,7 +9,7 @@
 //
 // fp16 inputs: P and dS have to be fp16 operands, whose normal range ends at 2^-14.  P (at most 1) is taken times 2^14
 // (kBiasFp16, added to the exponent), and dS further times a power of two per (batch, head) that keeps the bound
-// |dS| <= 2 max|dO row| max|V row| below 2^15; the factors are taken out of the sums in the epilogue.
+// |dS| <= 2 max|dO row| max|V row| (finite rows, keys that take part) below 2^15; the factors are taken out of the sums in the epilogue.
 #pragma once
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>

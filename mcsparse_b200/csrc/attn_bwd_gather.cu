@@ -578,7 +578,7 @@ int launch_db(AttnBwdParams& p, int heads_per_pass, cudaStream_t stream) {
 
 }  // namespace
 
-int launch_attn_bwd_gather_dkv(AttnBwdParams& p, bool fp16, int segs, int heads_per_pass, cudaStream_t stream) {
+int launch_attn_bwd_gather_rows(const AttnBwdParams& p, int segs, cudaStream_t stream) {
   const int bh = p.B * p.H;
   if (cudaMemsetAsync(p.seg_count, 0, (size_t)bh * segs * p.Sk * 4, stream) != cudaSuccess) return -8;
   const dim3 key_blocks((unsigned)((p.Sk + 1023) / 1024), (unsigned)bh);
@@ -586,6 +586,10 @@ int launch_attn_bwd_gather_dkv(AttnBwdParams& p, bool fp16, int segs, int heads_
   attn_bwd_block_sum_kernel<<<key_blocks, 1024, 0, stream>>>(p, segs);
   attn_bwd_scan_kernel<<<key_blocks, 1024, 0, stream>>>(p, segs);
   attn_bwd_rows_kernel<<<dim3((unsigned)segs, (unsigned)bh), 1024, 0, stream>>>(p, segs);
+  return cudaGetLastError() == cudaSuccess ? 0 : -8;
+}
+
+int launch_attn_bwd_gather_dkv(AttnBwdParams& p, bool fp16, int heads_per_pass, cudaStream_t stream) {
   const int blocks = p.D <= 64 ? 1 : (p.D <= 128 ? 2 : 4);
   if (fp16) return blocks == 1 ? launch_db<1, true>(p, heads_per_pass, stream) : (blocks == 2 ? launch_db<2, true>(p, heads_per_pass, stream) : launch_db<4, true>(p, heads_per_pass, stream));
   return blocks == 1 ? launch_db<1, false>(p, heads_per_pass, stream) : (blocks == 2 ? launch_db<2, false>(p, heads_per_pass, stream) : launch_db<4, false>(p, heads_per_pass, stream));

@@ -198,7 +198,8 @@ struct AttnBwdParams {
   int bh0, bh_count;                          // heads of this launch
 };
 int64_t attn_bwd_workspace_bytes(const AttnBwdParams& p, bool gather, bool fp16);
-int launch_attn_bwd_gather_dkv(AttnBwdParams& p, bool fp16, int segs, int heads_per_pass, cudaStream_t stream);
+int launch_attn_bwd_gather_rows(const AttnBwdParams& p, int segs, cudaStream_t stream);
+int launch_attn_bwd_gather_dkv(AttnBwdParams& p, bool fp16, int heads_per_pass, cudaStream_t stream);
 int launch_attn_bwd(AttnBwdParams& p, bool gather, bool fp16, void* workspace, cudaStream_t stream);
 
 // Sequence-to-head reshard by peer stores (see reshard.cu)
