@@ -33,8 +33,8 @@ def readable(t: Tensor) -> Tensor:
 
 def gradient_like(t: Tensor) -> Tensor:
     """Memory for the gradient of ``t``, in its layout where that one's rows are contiguous."""
-    return torch.empty_like(t, requires_grad=False) if t.stride(3) == 1 else torch.empty_like(t, memory_format=torch.contiguous_format,
-                                                                                             requires_grad=False)
+    g = torch.empty_like(t, requires_grad=False)             # (of windows, stride 1 twice, the rows may not be)
+    return g if g.stride(3) == 1 else torch.empty_like(t, memory_format=torch.contiguous_format, requires_grad=False)
 
 
 def launch_backward(entry: str, dout: Tensor, q: Tensor, k: Tensor, v: Tensor, out: Tensor, lse: Tensor, dq: Tensor, dk: Tensor, dv: Tensor,

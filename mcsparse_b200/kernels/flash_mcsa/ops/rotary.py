@@ -156,7 +156,7 @@ class RotaryEmbedding:
             src = outs = tuple(tensors)
         else:
             src = tuple(t if t.stride(3) == 1 else t.contiguous() for t in tensors)
-            outs = tuple(torch.empty_like(t, requires_grad=False) for t in src)
+            outs = tuple(_memory_like(t) for t in src)
         x, y = src[0], outs[0]
         B, L, H = x.shape[:3]
         if B == 0 or L == 0:
@@ -205,6 +205,12 @@ class RotaryEmbedding:
         """Gradients of the rotated tensors' inputs from those of the outputs: the rotation the other way, same magnitude."""
         outs = self._launch(grads, positions, True, inplace)
         return outs[0] if len(grads) == 1 else outs
+
+
+def _memory_like(t: Tensor) -> Tensor:
+    """Memory for the rotated ``t``: its order of dimensions, rows contiguous."""
+    y = torch.empty_like(t, requires_grad=False)             # (of windows, stride 1 twice, the rows may not be)
+    return y if y.stride(3) == 1 else torch.empty_like(t, memory_format=torch.contiguous_format, requires_grad=False)
 
 
 def _overlaps_itself(t: Tensor) -> bool:

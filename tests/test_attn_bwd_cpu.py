@@ -123,3 +123,10 @@ def test_oracle_gradients_by_autograd():
     grads, bounds = head_grads(q, k, v, dout, out.detach(), 0.25, torch.bfloat16, hide)
     for a, b, t in zip(grads, want, bounds):
         assert torch.allclose(a, b, rtol=1e-12, atol=1e-12) and bool((t > 0).any())
+
+
+def test_gradients_have_contiguous_rows_whatever_the_input():
+    x = torch.zeros(1000, dtype=torch.bfloat16)
+    for shape, stride in [((1, 2, 4, 16), (0, 104, 1, 1)), ((2, 4, 2, 16), (304, 1, 64, 1)), ((2, 4, 2, 16), (304, 16, 16, 1))]:
+        y = attn_bwd.gradient_like(x.as_strided(shape, stride))
+        assert y.shape == shape and y.stride(3) == 1 and all(s % 8 == 0 for s in y.stride()[:3])

@@ -7,6 +7,7 @@ import pytest
 import torch
 
 from mcsparse_b200 import _lib
+from mcsparse_b200.kernels.flash_mcsa.ops import rotary as rotary_module
 from mcsparse_b200.h3.ulysses_layer import rope_pairs
 from mcsparse_b200.kernels.flash_mcsa.ops.rotary import RotaryEmbedding
 
@@ -113,3 +114,14 @@ def test_entry_point_refusals():
     a = args()
     a.H[0] = 0
     assert lib.mcs_rotary(a, None) == 0
+
+
+def test_results_have_contiguous_rows_whatever_the_input():
+    """Windows of a sequence (a stride of one twice): memory in the input's order of strides would put the window, not the head, last."""
+    x = torch.zeros(1000)
+    for shape, stride in [((1, 2, 4, 16), (0, 100, 1, 1)), ((2, 4, 2, 16), (300, 1, 64, 1)), ((2, 4, 2, 16), (300, 64, 16, 1))]:
+        t = x.as_strided(shape, stride)
+        y = rotary_module._memory_like(t)
+        assert y.shape == t.shape and y.stride(3) == 1 and not rotary_module._overlaps_itself(y)
+    t = torch.zeros(2, 3, 5, 16).transpose(1, 2)
+    assert rotary_module._memory_like(t).stride() == t.stride()
