@@ -106,8 +106,20 @@ class RotaryEmbedding:
                 freq.append(f)
                 axis.append(a)
         self.frequencies, self.pair_axis = tuple(freq), tuple(axis)
-        self._turns = (C.c_uint64 * len(freq))(*[_turns(f) for f in freq])
-        self._axis = (C.c_uint8 * len(axis))(*axis)
+        self._lay_out()
+
+    def _lay_out(self) -> None:
+        """The arrays that a launch copies into its arguments."""
+        n = len(self.frequencies)
+        self._turns = (C.c_uint64 * n)(*[_turns(f) for f in self.frequencies])
+        self._axis = (C.c_uint8 * n)(*self.pair_axis)
+
+    def __getstate__(self):
+        return {k: x for k, x in self.__dict__.items() if k not in ("_turns", "_axis")}
+
+    def __setstate__(self, state) -> None:
+        self.__dict__.update(state)
+        self._lay_out()
 
     # ------------------------------------------------------------------------------------------ launches
     def _check(self, tensors: Sequence[Tensor], positions: Tensor) -> Tuple[int, int, int]:
@@ -151,8 +163,8 @@ class RotaryEmbedding:
             for t in tensors:
                 if t.stride(-1) != 1 or _overlaps_itself(t):
                     raise ValueError("inplace needs tensors with contiguous rows whose elements do not share memory")
-            if len(tensors) == 2 and tensors[0].data_ptr() == tensors[1].data_ptr() and tensors[0].numel() > 0:
-                raise ValueError("inplace needs two different tensors")
+            if len(tensors) == 2 and _may_share(*tensors):
+                raise ValueError("inplace needs two tensors that share no element")
             src = outs = tuple(tensors)
         else:
             src = tuple(t if t.stride(3) == 1 else t.contiguous() for t in tensors)
@@ -188,7 +200,7 @@ class RotaryEmbedding:
         """Rotated copies of one or two (B, L, H, D) tensors (q and k; the head counts may differ), from one launch.
 
         ``positions``: int32 or int64 on the tensors' device, any strides: (L,) or (B, L) for one axis, (L, axes) or
-        (B, L, axes) for several.  Differentiable in the tensors.  ``inplace`` overwrites them instead (forward only).
+        (B, L, axes) for several.  Differentiable in the tensors.  ``inplace`` overwrites them instead (forward only; they share no element).
         Returns a tensor for one, a tuple for two."""
         if torch.is_grad_enabled() and any(t.requires_grad for t in tensors):
             if inplace:
@@ -221,6 +233,33 @@ def _overlaps_itself(t: Tensor) -> bool:
             return True
         end = stride * (size - 1) + end
     return False
+
+
+def _may_share(a: Tensor, b: Tensor) -> bool:
+    """Whether a and b, neither overlapping itself, may have an element in common.  Views of one layout are told apart (heads of a packed
+    projection, say); others count as sharing where their ranges of addresses meet."""
+    if a.numel() == 0 or b.numel() == 0:
+        return False
+    if a.data_ptr() > b.data_ptr():
+        a, b = b, a
+    extent = lambda t, dims: 1 + sum(t.stride(d) * (t.shape[d] - 1) for d in dims)
+    size, offset = a.element_size(), b.data_ptr() - a.data_ptr()
+    if offset >= size * extent(a, range(4)):
+        return False
+    dims = [d for d in range(4) if a.shape[d] > 1 or b.shape[d] > 1]
+    if offset % size or any(a.stride(d) != b.stride(d) and a.shape[d] > 1 and b.shape[d] > 1 for d in dims):
+        return True
+    offset //= size
+    stride = {d: a.stride(d) if a.shape[d] > 1 else b.stride(d) for d in dims}
+    order = sorted(dims, key=stride.get)
+    for i, d in enumerate(order):
+        # modulo a stride that divides all greater ones only the lesser dimensions and the offset remain: apart if those are
+        step, inner = stride[d], order[:i]
+        if step and all(stride[e] % step == 0 for e in order[i:]):
+            rest = offset % step
+            if extent(a, inner) <= rest and rest + extent(b, inner) <= step:
+                return False
+    return True
 
 
 class _Rotate(torch.autograd.Function):

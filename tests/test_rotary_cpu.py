@@ -125,3 +125,47 @@ def test_results_have_contiguous_rows_whatever_the_input():
         assert y.shape == t.shape and y.stride(3) == 1 and not rotary_module._overlaps_itself(y)
     t = torch.zeros(2, 3, 5, 16).transpose(1, 2)
     assert rotary_module._memory_like(t).stride() == t.stride()
+
+
+def test_tensors_that_share_elements_are_told_from_slices_of_one_projection():
+    """Against sets of element offsets, over slices of packed projections and shifted views."""
+    base = torch.zeros(4000)
+
+    def offsets(t):
+        at = t.storage_offset() + sum(torch.arange(n).view([-1 if i == d else 1 for i in range(4)]) * s for d, (n, s) in enumerate(zip(t.shape, t.stride())))
+        return set(at.flatten().tolist())
+    packed, heads = base[:2 * 5 * 7 * 8].view(2, 5, 7, 8), base[:2 * 6 * 5 * 8].view(2, 6, 5, 8).transpose(1, 2)
+    three = base[:2 * 5 * 3 * 2 * 8].view(2, 5, 3, 2, 8)
+    apart = [(packed[:, :, :4], packed[:, :, 4:6]), (packed[:, :, 5:], packed[:, :, :3]), (heads[:, :, :3], heads[:, :, 3:]), (packed[:1], packed[1:]),
+             (three[:, :, 0], three[:, :, 1]), (three[:, :, 2], three[:, :, 0]), (packed[:, :, :, :4], packed[:, :, :, 4:]),
+             (packed[:, :4, :4], packed[:, 1:, 4:]), (packed[:, :, :1], packed[:, :, 1:]), (packed[:, :, :0], packed), (base[:320].view(2, 5, 4, 8), base[320:640].view(2, 5, 4, 8))]
+    share = [(packed, packed), (packed[:, :, :4], packed[:, :, 3:]), (packed[:, :4], packed[:, 1:]), (packed[:, :, :4], packed[:, :, 2:6]),
+             (heads[:, :, :3], heads[:, :, 2:5]), (packed[..., :5], packed[..., 3:]), (base[:320].view(2, 5, 4, 8), base[8:328].view(2, 5, 4, 8)),
+             (base[:320].view(2, 5, 4, 8), base[:320].view(2, 4, 5, 8).transpose(1, 2))]
+    for a, b in apart:
+        assert not offsets(a) & offsets(b)
+        assert not rotary_module._may_share(a, b) and not rotary_module._may_share(b, a)
+    for a, b in share:
+        assert offsets(a) & offsets(b)
+        assert rotary_module._may_share(a, b) and rotary_module._may_share(b, a)
+    # never missed, whatever the strides
+    g = torch.Generator().manual_seed(0)
+    pick = lambda n: int(torch.randint(0, n, (1,), generator=g))
+    for _ in range(600):
+        shape = [(1 + pick(3), 1 + pick(4), 1 + pick(3), 4) for _ in range(2)]
+        strides = (pick(60), pick(30), pick(16), 1)
+        a, b = (base.as_strided(s, strides, pick(80)) for s in shape)
+        if rotary_module._overlaps_itself(a) or rotary_module._overlaps_itself(b):
+            continue
+        if offsets(a) & offsets(b):
+            assert rotary_module._may_share(a, b), (a.shape, b.shape, strides, a.storage_offset(), b.storage_offset())
+
+
+def test_plan_is_copied_and_stored_with_a_module():
+    import copy
+    import pickle
+    plan = RotaryEmbedding(32, rotary_dim=16, axis_pairs=(4, 4), layout="half", scaling="linear", factor=2.0)
+    for other in (copy.deepcopy(plan), pickle.loads(pickle.dumps(plan))):
+        assert list(other._turns) == list(plan._turns) and list(other._axis) == list(plan._axis)
+        assert C.addressof(other._turns) != C.addressof(plan._turns)
+        assert other.frequencies == plan.frequencies and other.layout == plan.layout and other.magnitude == plan.magnitude
