@@ -60,7 +60,7 @@ __global__ void __launch_bounds__(256) attn_bwd_stats_kernel(const AttnBwdParams
     for (int u = 0; u < kRows; ++u) {
       const int i = base + u * 16 + sub, r = i & 127, pos = (i >> 7) * p.group_rows + r;
       row[u] = -1;
-      if (i < rows && r < p.group_rows && pos < p.Sq) row[u] = p.perm != nullptr ? (int)p.perm[(size_t)bh * p.Sq + pos] : pos;
+      if (i < rows && r < p.group_rows && pos < p.Sq) row[u] = query_row(p, bh, pos);
     }
     for (int c = l16; c < chunks; c += 16) {
       uint4 x[kRows], y[kRows];
@@ -252,7 +252,7 @@ __global__ void __launch_bounds__(threads_of(kMode), 1) attn_bwd_kernel(const At
     } else {
       const int pos = it.m * p.group_rows + r;
       if (r >= p.group_rows || pos >= p.Sq) return -1;
-      return p.perm != nullptr ? (int)p.perm[(size_t)it.bh * p.Sq + pos] : pos;
+      return query_row(p, it.bh, pos);
     }
   };
 

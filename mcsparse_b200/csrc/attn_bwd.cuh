@@ -23,6 +23,14 @@ namespace bwd {
 constexpr float kBiasFp16 = 14.f;
 constexpr int kSoftmaxWarps = 8;       // warps 0-3 take the first half of a score tile's columns, 4-7 the second; lane == row
 
+// Row of q, out, dout and dq at position pos < Sq of head bh's order; -1, a row that is not there, for an entry of perm out of range: what
+// is written through it must stay inside dq.
+__device__ __forceinline__ int query_row(const AttnBwdParams& p, int bh, int pos) {
+  if (p.perm == nullptr) return pos;
+  const int64_t row = p.perm[(size_t)bh * p.Sq + pos];
+  return row >= 0 && row < p.Sq ? (int)row : -1;
+}
+
 // Power of two by which dS / 2^14 may be multiplied (see above), from the largest row norms; 1 for bf16.  A whole warp calls it.
 constexpr int kMaxBlocks = 64;          // CTAs per head of the statistics, each of which leaves its own maxima
 template <bool kFp16>

@@ -167,7 +167,7 @@ __global__ void __launch_bounds__(kThreadsG, 1) attn_bwd_gather_dkv_kernel(const
   auto row_of = [&](const Item& it, int r) {
     const int pos = it.m * p.group_rows + r;
     if (r >= p.group_rows || pos >= p.Sq) return -1;
-    return p.perm != nullptr ? (int)p.perm[(size_t)it.bh * p.Sq + pos] : pos;
+    return query_row(p, it.bh, pos);
   };
 
   if (tid == 0) {

@@ -184,3 +184,21 @@ def test_neighbouring_memory_is_left_alone(cuda_device):
             assert torch.equal(w, r)
             w.fill_(7.0)
             assert bool((b == 7.0).all())
+
+
+def test_entries_of_perm_out_of_range_take_no_part(cuda_device):
+    """Bounds-checked in every kernel that follows perm: nothing outside the tensors is read or written."""
+    c = make(1, 2, 300, 400, 64, 128, torch.bfloat16, cuda_device, perm=True)
+    kw = dict(gather_kv_lengths=c["gl"], group_rows=c["rows"])
+    out, lse = flash_attn_gather_kv_func(c["q"], c["k"], c["v"], c["gi"], return_lse=True, perm=c["perm"], **kw)
+    gone, bad = c["perm"][:, 5].clone(), c["perm"].clone()
+    bad[0, 5], bad[1, 5] = 300, -1
+    dout = c["dout"].clone()
+    for h in range(2):
+        dout[0, gone[h], h] = 0                              # a row without gradient from above adds nothing to dk and dv
+    want = flash_attn_gather_kv_backward_func(dout, c["q"], c["k"], c["v"], out, lse, c["gi"], perm=c["perm"], **kw)
+    got = flash_attn_gather_kv_backward_func(c["dout"], c["q"], c["k"], c["v"], out, lse, c["gi"], perm=bad, **kw)
+    for h in range(2):
+        others = torch.arange(300, device=cuda_device) != gone[h]
+        assert torch.equal(got[0][0, others, h], want[0][0, others, h])
+    assert torch.equal(got[1], want[1]) and torch.equal(got[2], want[2])
