@@ -167,6 +167,12 @@ __global__ void __launch_bounds__(256) attn_bwd_stats_kernel(const AttnBwdParams
 // kernel therefore sums the rounded dS, and PK = sum_j P_ij K_j beside dQ, and stores dQ - r PK: 2.3e-3.  The fourth product takes
 // the tensor pipe as long as the kernel of dK and dV does.  The sum of dS before rounding, too, is taken: it is what delta is off
 // by, and the key side, which runs second, gets delta without it (dK: 2.7e-3 -> 2.4e-3 with lists of selected keys).
+//
+// Short sums (kPaired; see pick_paired): the rounding of P and dS does not average out over a few rows, and
+// where these resemble one another (neighbouring tokens) the sums cancel and the rounding does not: 7 queries on 33 keys x 64, bf16: error of dK
+// 3.5e-3 of its norm, 1.6e-3 of it the result's own rounding.  A tile then holds TN / 2 rows twice, and the second half of the softmax
+// threads stores what the first half's rounding left, so that the sums take P and dS with twice the bits.  Up to TN / 2 rows this fills
+// what would be padding.
 enum { kDq = 0, kDqGather = 1, kDkv = 2 };
 
 template <int DB, int TN>
@@ -198,13 +204,15 @@ constexpr int threads_of(int mode) { return mode == kDqGather ? 32 * (kLoadWarp0
 // Blocks of output columns: one, or two of 128 where tensor memory does not hold both sums at full width.
 __host__ __device__ constexpr int column_blocks(int D) { return D > 192 ? 2 : 1; }
 
-template <int DB, int TN, bool kFp16, int kMode>
+template <int DB, int TN, bool kFp16, int kMode, bool kPaired>
 __global__ void __launch_bounds__(threads_of(kMode), 1) attn_bwd_kernel(const AttnBwdParams p, const __grid_constant__ DenseTileMaps maps,
                                                                 const __grid_constant__ DenseTileMaps res) {
   using L = SmemB<DB, TN>;
   using G = Geo<DB, TN>;
   constexpr bool kGather = kMode == kDqGather, kRowsAreKeys = kMode == kDkv;
   constexpr int R = L::kRing, HC = G::kHalf;
+  constexpr int TR = kPaired ? HC : TN;                      // different rows of a streamed tile
+  static_assert(!kPaired || !kGather, "lists of keys are longer");
   // (no room for a manual alignment: the tiles need 1,024 bytes, which the declaration asks for and the host would be told if it failed)
   extern __shared__ __align__(1024) uint8_t smem[];
   const uint32_t s_base = smem_u32(smem);
@@ -238,7 +246,7 @@ __global__ void __launch_bounds__(threads_of(kMode), 1) attn_bwd_kernel(const At
       const int most = p.gather_len / 128;
       T = (p.gl != nullptr ? min(max(p.gl[(size_t)it.bh * p.M + it.m], 1), most) : most) * (128 / TN);
     } else {
-      T = ((kRowsAreKeys ? p.Sq : p.Sk) + TN - 1) / TN;
+      T = ((kRowsAreKeys ? p.Sq : p.Sk) + TR - 1) / TR;
     }
     it.t0 = (int)((long long)T * it.split / p.splits);
     it.t1 = (int)((long long)T * (it.split + 1) / p.splits);
@@ -337,7 +345,7 @@ __global__ void __launch_bounds__(threads_of(kMode), 1) attn_bwd_kernel(const At
         }
         if constexpr (kMode == kDq) {
           // key positions behind the sequence end (zero rows of the last tile): exp2(-lse2) could be anything
-          const int rem = p.Sk - t * TN - x * HC;
+          const int rem = p.Sk - t * TR - (kPaired ? 0 : x * HC);
           if (rem < HC) {
 #pragma unroll
             for (int i = 0; i < HC; ++i)
@@ -356,7 +364,21 @@ __global__ void __launch_bounds__(threads_of(kMode), 1) attn_bwd_kernel(const At
         load_columns<kStep>(tDP, dp);
         tmem_wait_ld();
 #pragma unroll
-        for (int q = 0; q < HC / 16; ++q) store_packed<kFp16>(tDP + q * 8, &sc[q * 16]);
+        for (int q = 0; q < HC / 16; ++q) {
+          if (kPaired && x == 1) {
+            uint32_t rest[16];
+#pragma unroll
+            for (int i = 0; i < 16; i += 2) {
+              float a = __uint_as_float(sc[q * 16 + i]), b = __uint_as_float(sc[q * 16 + i + 1]);
+              keep_rest<kFp16>(a, b);
+              rest[i] = __float_as_uint(a);
+              rest[i + 1] = __float_as_uint(b);
+            }
+            store_packed<kFp16>(tDP + q * 8, rest);
+          } else {
+            store_packed<kFp16>(tDP + q * 8, &sc[q * 16]);
+          }
+        }
         tmem_wait_st();
         tc_fence_before();
         warp_arrive(bar(L::kPReady));
@@ -377,12 +399,18 @@ __global__ void __launch_bounds__(threads_of(kMode), 1) attn_bwd_kernel(const At
             if constexpr (kFp16) { d0 = f2_mul(d0, c2); d1 = f2_mul(d1, c2); }
             d0 = f2_mul(f2_pack(__uint_as_float(sc[e]), __uint_as_float(sc[e + 1])), d0);
             d1 = f2_mul(f2_pack(__uint_as_float(sc[e + 2]), __uint_as_float(sc[e + 3])), d1);
-            const float2 y0 = f2_unpack(d0), y1 = f2_unpack(d1);
+            float2 y0 = f2_unpack(d0), y1 = f2_unpack(d1);
+            if (kPaired && x == 1) {
+              keep_rest<kFp16>(y0.x, y0.y);
+              keep_rest<kFp16>(y1.x, y1.y);
+            }
             pk[d / 2] = pack16<kFp16>(y0.x, y0.y);
             pk[d / 2 + 1] = pack16<kFp16>(y1.x, y1.y);
             if constexpr (!kRowsAreKeys) {
-              es[0] = f2_add(es[0], d0);
-              es[1] = f2_add(es[1], d1);
+              if (!kPaired || x == 0) {
+                es[0] = f2_add(es[0], d0);
+                es[1] = f2_add(es[1], d1);
+              }
               add_pair<kFp16>(pk[d / 2], rs[0], rs[1]);
               add_pair<kFp16>(pk[d / 2 + 1], rs[2], rs[3]);
             }
@@ -707,13 +735,16 @@ __global__ void __launch_bounds__(threads_of(kMode), 1) attn_bwd_kernel(const At
           mbar_arrive_expect_tx(bar(L::kFull + slot), G::kTileBytes + (kRowsAreKeys ? TN * 4 : 0));
           const void* map = is_t1 ? static_cast<const void*>(maps.v) : static_cast<const void*>(maps.k);
           int co[4] = {0, is_t1 ? c1[1] : c0[1], is_t1 ? c1[2] : c0[2], is_t1 ? c1[3] : c0[3]};
-          co[is_t1 ? maps.v_pos_row : maps.k_pos_row] = (e >> 1) * TN;
+          co[is_t1 ? maps.v_pos_row : maps.k_pos_row] = (e >> 1) * TR;
 #pragma unroll
-          for (int cb = 0; cb < DB; ++cb)
-            tma_load_4d(sRing(slot) + cb * TN * 128, map, cb * 64, co[1], co[2], co[3], bar(L::kFull + slot));
-          if constexpr (kRowsAreKeys)
-            bulk_load(s_base + L::kStat + slot * TN * 4, (is_t1 ? p.neg_delta_kv : p.neg_lse2) + (size_t)it.bh * p.stat_rows + (size_t)(e >> 1) * TN, TN * 4,
-                      bar(L::kFull + slot));
+          for (int half = 0; half < TN / TR; ++half) {       // (boxes of TR rows)
+#pragma unroll
+            for (int cb = 0; cb < DB; ++cb)
+              tma_load_4d(sRing(slot) + (cb * TN + half * TR) * 128, map, cb * 64, co[1], co[2], co[3], bar(L::kFull + slot));
+            if constexpr (kRowsAreKeys)
+              bulk_load(s_base + L::kStat + (slot * TN + half * TR) * 4,
+                        (is_t1 ? p.neg_delta_kv : p.neg_lse2) + (size_t)it.bh * p.stat_rows + (size_t)(e >> 1) * TR, TR * 4, bar(L::kFull + slot));
+          }
         }
       }
     }
@@ -780,7 +811,7 @@ int sm_count() {
 
 // Splits of the summed axis (T tiles) for `items` items without splits, whose partial sums are `part_bytes` per split.  Measured
 // at 1.9 GHz: a tile takes tile_us; an item besides 3.5 us to fill, drain and store (5.5 us with fp32 partial sums); the kernel that
-// adds the partial sums reads them at 4.3 TB/s and costs 2.5 us to launch.
+// adds the partial sums reads them at 4.3 TB/s and takes 5.5 us besides (2 heads x 257 x 64: dQ's 5.3, dK's and dV's together 5.9).
 int pick_splits(long long items, int T, double tile_us, double part_bytes) {
   // (for the B200's 148 SMs, whatever the current device: the workspace must not depend on the device that asks)
   constexpr int kSms = 148;
@@ -788,7 +819,7 @@ int pick_splits(long long items, int T, double tile_us, double part_bytes) {
   int pick = 1;
   for (int s = 1; s <= T && s <= 32; ++s) {
     const double waves = (double)((items * s + kSms - 1) / kSms);
-    const double us = waves * ((T + s - 1) / s * tile_us + (s > 1 ? 5.5 : 3.5)) + (s > 1 ? 2.5 + s * part_bytes / 4.3e6 : 0.0);
+    const double us = waves * ((T + s - 1) / s * tile_us + (s > 1 ? 5.5 : 3.5)) + (s > 1 ? 5.5 + s * part_bytes / 4.3e6 : 0.0);
     if (s == 1 || us < best) { best = us; pick = s; }
   }
   return pick;
@@ -798,10 +829,16 @@ int pick_splits(long long items, int T, double tile_us, double part_bytes) {
 // passes would only add launches with a partly filled last wave.
 constexpr size_t kPartsBytes = 4ull << 30;
 
-struct Plan { int stat_rows, dq_splits, kv_splits, segs, heads_per_pass; size_t stats, row_max, entries, starts, counts, blocks, parts, total; };
+struct Plan { bool pair_k, pair_q; int stat_rows, dq_splits, kv_splits, segs, heads_per_pass; size_t stats, row_max, entries, starts, counts, blocks, parts, total; };
 
 constexpr size_t kAlign = 256;
 size_t up(size_t n) { return (n + kAlign - 1) / kAlign * kAlign; }
+
+// Whether tiles of a streamed axis of S rows hold their rows twice: up to 64 rows, where that fills padding (D <= 128), and up to 256
+// where the tiles, now twice as many, are no more than the SMs, most of which would be idle.  Errors of dK relative to the result's own
+// rounding, 65 to 130 queries on 33 to 90 keys: 1.51 to 1.56 without, 1.00 with it.  Time of a captured call of 128 x 128 x 128: 17.9 and 21.6 us;
+// of 4 heads x 512 x 512 x 128 26.2 and 33.7, for sums over which the rounding averages out (1.4): not taken there.
+bool pick_paired(long long items, int S, int TN) { return S <= 64 || (S <= 256 && items * ((S + TN / 2 - 1) / (TN / 2)) <= 148); }
 
 // Rows of a streamed tile: as many as tensor memory holds beside both sums, and shared memory beside the resident tiles.  (96 rows up to
 // D = 160 would fit, with a ring of three tiles instead of five: 18,944 x 144 took 488 us a side against 455.)
@@ -819,8 +856,12 @@ Plan make_plan(const AttnBwdParams& p, bool gather) {
     w.dq_splits = w.kv_splits = 1;
   } else {
     const double tile_us = p.D <= 64 ? 1.3 : (p.D <= 128 ? 1.6 : 1.2);
-    w.dq_splits = pick_splits(bh * p.M * blocks, (p.Sk + TN - 1) / TN, tile_us, (double)bh * p.Sq * (2 * p.D + 8) * 4);
-    w.kv_splits = pick_splits(bh * ((p.Sk + 127) / 128) * blocks, (p.Sq + TN - 1) / TN, tile_us, (double)bh * p.Sk * 2 * p.D * 4);
+    const long long q_items = bh * p.M * blocks, k_items = bh * ((p.Sk + 127) / 128) * blocks;
+    w.pair_k = pick_paired(q_items, p.Sk, TN);
+    w.pair_q = pick_paired(k_items, p.Sq, TN);
+    const int tk = w.pair_k ? TN / 2 : TN, tq = w.pair_q ? TN / 2 : TN;
+    w.dq_splits = pick_splits(q_items, (p.Sk + tk - 1) / tk, tile_us, (double)bh * p.Sq * (2 * p.D + 8) * 4);
+    w.kv_splits = pick_splits(k_items, (p.Sq + tq - 1) / tq, tile_us, (double)bh * p.Sk * 2 * p.D * 4);
   }
   w.stat_rows = p.M * 128;
   w.stats = up((size_t)bh * w.stat_rows * 4);
@@ -855,20 +896,22 @@ int set_smem(K kern, int bytes) {
 
 template <int DB, int TN, bool kFp16>
 int launch_dense(AttnBwdParams& p, const Plan& w, cudaStream_t stream) {
-  // boxes of TN rows for streamed tiles, of 128 for resident ones
+  // boxes of TN rows (paired: half as many, twice) for streamed tiles, of 128 for resident ones
+  const int rows_k = w.pair_k ? TN / 2 : TN, rows_q = w.pair_q ? TN / 2 : TN;
   auto maps = [&](DenseTileMaps& m, const void* a, const int64_t* as, const void* b, const int64_t* bs, int S, int rows) {
     return encode_tile_map(a, as, p.B, S, p.H, p.D, m.k, m.k_pos_h, m.k_pos_row, m.k_pos_b, rows) &&
            encode_tile_map(b, bs, p.B, S, p.H, p.D, m.v, m.v_pos_h, m.v_pos_row, m.v_pos_b, rows);
   };
   DenseTileMaps kv, qd, res_kv, res_qd;
-  if (!maps(kv, p.k, p.k_stride, p.v, p.v_stride, p.Sk, TN) || !maps(qd, p.q, p.q_stride, p.dout, p.dout_stride, p.Sq, TN)) return -9;
+  if (!maps(kv, p.k, p.k_stride, p.v, p.v_stride, p.Sk, rows_k) || !maps(qd, p.q, p.q_stride, p.dout, p.dout_stride, p.Sq, rows_q)) return -9;
   res_kv = kv;
   res_qd = qd;
-  if (TN != 128 && (!maps(res_kv, p.k, p.k_stride, p.v, p.v_stride, p.Sk, 128) || !maps(res_qd, p.q, p.q_stride, p.dout, p.dout_stride, p.Sq, 128))) return -9;
+  if (rows_k != 128 && !maps(res_kv, p.k, p.k_stride, p.v, p.v_stride, p.Sk, 128)) return -9;
+  if (rows_q != 128 && !maps(res_qd, p.q, p.q_stride, p.dout, p.dout_stride, p.Sq, 128)) return -9;
   const int sms = sm_count();
   const long long bh = (long long)p.B * p.H;
-  auto dq = attn_bwd_kernel<DB, TN, kFp16, kDq>;
-  auto dkv = attn_bwd_kernel<DB, TN, kFp16, kDkv>;
+  auto dq = w.pair_k ? attn_bwd_kernel<DB, TN, kFp16, kDq, true> : attn_bwd_kernel<DB, TN, kFp16, kDq, false>;
+  auto dkv = w.pair_q ? attn_bwd_kernel<DB, TN, kFp16, kDkv, true> : attn_bwd_kernel<DB, TN, kFp16, kDkv, false>;
   constexpr int kSmem = SmemB<DB, TN>::kDynamic;
   if (set_smem(dq, kSmem) || set_smem(dkv, kSmem)) return -8;
   const int blocks = column_blocks(p.D);
@@ -895,7 +938,7 @@ int launch_dense(AttnBwdParams& p, const Plan& w, cudaStream_t stream) {
 
 template <int DB, int TN, bool kFp16>
 int launch_gather_dq(AttnBwdParams& p, cudaStream_t stream) {
-  auto dq = attn_bwd_kernel<DB, TN, kFp16, kDqGather>;
+  auto dq = attn_bwd_kernel<DB, TN, kFp16, kDqGather, false>;
   constexpr int kSmem = SmemB<DB, TN>::kDynamic;
   if (set_smem(dq, kSmem)) return -8;
   const int sms = sm_count();

@@ -133,6 +133,20 @@ __device__ __forceinline__ void store_packed(uint32_t taddr, const uint32_t* v) 
   tmem_st8(taddr, pk);
 }
 
+// what rounding a and b to 16 bits leaves of them
+template <bool kFp16>
+__device__ __forceinline__ void keep_rest(float& a, float& b) {
+  const uint32_t u = pack16<kFp16>(a, b);
+  if constexpr (kFp16) {
+    const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&u));
+    a -= f.x;
+    b -= f.y;
+  } else {
+    a -= bf16_lo(u);
+    b -= bf16_hi(u);
+  }
+}
+
 // eight fp32 values as one 32-byte store: a row's thread fills whole sectors
 __device__ __forceinline__ void store8(float* dst, const float* f) {
   asm volatile("st.global.v8.f32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(dst), "f"(f[0]), "f"(f[1]), "f"(f[2]), "f"(f[3]), "f"(f[4]), "f"(f[5]),

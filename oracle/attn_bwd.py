@@ -16,7 +16,8 @@ with fp32 products and sums, P and dS rounded once to the input type (relative s
   PK = P K: beside sum err(dS) |K| at most sum err(dS) times P |K|;
 * fp16: P and dS are scaled by powers of two such that the half-step of the smallest fp16 numbers, 2^-25, stands for less than
   2^-39 of P's largest value 1 and of the bound 2 max|dO| max|V| of dS;
-* the result's own rounding, u of its value.
+* the result's own rounding, u of its value;
+* where an axis is short the kernel takes P and dS as two 16-bit parts each, the rounded value and the rounded rest: u becomes u^2 (`paired`).
 """
 
 from __future__ import annotations
@@ -26,10 +27,12 @@ import math
 import torch
 
 
-def head_grads(q, k, v, dout, out, scale, dtype, hide=None):
+def head_grads(q, k, v, dout, out, scale, dtype, hide=None, paired=False):
     """One head, 64-bit (n, D) queries and (m, D) keys: (dq, dk, dv) and their bounds before the final rounding.  `hide`: bool (n, m),
     keys that a query does not see.  `dtype`: the kernel's input type."""
     u = torch.finfo(dtype).eps / 2
+    if paired:
+        u = u * u
     s = scale * (q @ k.t())
     if hide is not None:
         s = s.masked_fill(hide, -math.inf)
@@ -52,12 +55,12 @@ def head_grads(q, k, v, dout, out, scale, dtype, hide=None):
     return (dq, dk, dv), (tol_dq, tol_dk, err_dv.t() @ dout.abs())
 
 
-def dense_grads(q, k, v, dout, out, scale, dtype):
+def dense_grads(q, k, v, dout, out, scale, dtype, paired=False):
     """(B, H, L, D) tensors -> ((dq, dk, dv), bounds), in 64 bits on their device."""
     res = [torch.empty(t.shape, dtype=torch.float64, device=t.device) for t in (q, k, v, q, k, v)]
     for b in range(q.shape[0]):
         for h in range(q.shape[1]):
-            g, t = head_grads(*(x[b, h].double() for x in (q, k, v, dout, out)), scale, dtype)
+            g, t = head_grads(*(x[b, h].double() for x in (q, k, v, dout, out)), scale, dtype, paired=paired)
             for dst, src in zip(res, (*g, *t)):
                 dst[b, h] = src
     return res[:3], res[3:]
