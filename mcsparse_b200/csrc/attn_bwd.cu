@@ -435,7 +435,10 @@ __global__ void __launch_bounds__(threads_of(kMode), 1) attn_bwd_kernel(const At
       const float unbias = kFp16 ? 6.103515625e-05f : 1.f;                     // 2^-14
       float fix = 0.f, off = 0.f;
       if constexpr (!kRowsAreKeys) {
-        // the row's sums of dS from its two threads; the other's are read before this item's kOFree, so before they are written again
+        // The row's sums of dS from its two threads.  A thread arrives at kOFree behind its reads of the other's, and none writes here before
+        // all have arrived there for the item before: an item of one tile gets this far on S and dP, for which nobody waits for kOFree.
+        if (ic > 0) ok = mbar_wait(bar(L::kOFree), (ic - 1) & 1, p.status, 146);
+        if (!ok) break;
         float* sums = reinterpret_cast<float*>(smem + L::kStat);
         const float2 a2 = f2_unpack(es[0]), b2 = f2_unpack(es[1]);
         sums[x * 128 + r_in] = (rs[0] + rs[1]) + (rs[2] + rs[3]);

@@ -1,0 +1,201 @@
+"""The waits of the attention's backward kernel (csrc/attn_bwd.cu), modelled on the CPU.
+
+Every warp, or group of warps with one role, is a list of steps: wait for a phase of a barrier, arrive at one, write a place, read a place
+and find what was meant for it.  Barriers behave as the hardware's: a wait sees the parity of the running phase only, so a barrier that has
+moved two phases on looks as if it had not moved.  A run holds one warp up in front of one of its steps until nobody else can go on, then
+lets it go; every step of every warp is held up once.  No run may get stuck or read what was not meant for the reader.
+
+The model follows the kernel's program order by hand.  Each of its switches takes one of the kernel's waits away, and the model has to find
+what that wait is for.
+"""
+
+import pytest
+
+
+class Barrier:
+    def __init__(self, count):
+        self.count, self.pending, self.phases = count, count, 0
+
+    def arrive(self):
+        self.pending -= 1
+        if self.pending == 0:
+            self.pending, self.phases = self.count, self.phases + 1
+
+
+class Fault(Exception):
+    pass
+
+
+class Model:
+    def __init__(self):
+        self.counts, self.warps = {}, {}
+
+    def barrier(self, name, count):
+        self.counts[name] = count
+
+    def warp(self, name):
+        steps = self.warps[name] = []
+        return (lambda bar, phase: steps.append(("wait", bar, phase)), lambda bar: steps.append(("arrive", bar, None)),
+                lambda place, value: steps.append(("write", place, value)), lambda place, value: steps.append(("read", place, value)))
+
+    def run(self, held, at):
+        bars = {name: Barrier(n) for name, n in self.counts.items()}
+        places, pos = {}, dict.fromkeys(self.warps, 0)
+
+        def advance(name, stop):
+            """Steps of a warp until it has to wait; whether it took any."""
+            steps, first = self.warps[name], pos[name]
+            while pos[name] < stop:
+                op, what, value = steps[pos[name]]
+                if op == "wait" and bars[what].phases & 1 == value & 1:
+                    break
+                if op == "arrive":
+                    bars[what].arrive()
+                elif op == "write":
+                    places[what] = value
+                elif op == "read" and places.get(what) != value:
+                    raise Fault(f"{name} reads {what}: {places.get(what)} for {value} (held: {held} at {at})")
+                pos[name] += 1
+            return pos[name] > first
+
+        for stops in ({held: at}, {}):
+            while any([advance(name, stops.get(name, len(steps))) for name, steps in self.warps.items()]):
+                pass
+        stuck = {n: steps[pos[n]] for n, steps in self.warps.items() if pos[n] < len(steps)}
+        if stuck:
+            raise Fault(f"stuck (held: {held} at {at}): {stuck}")
+
+    def check(self):
+        for name, steps in self.warps.items():
+            for at in range(len(steps)):
+                self.run(name, at)
+
+
+def backward(items, keys, ordered, ring, ordered_sums=True):
+    """One CTA of attn_bwd_kernel that walks `items` (tiles of each).  `keys`: the mode of dK and dV, else that of dQ.  `ordered`: tiles of 128
+    rows, whose S and dP are issued in a fixed order.  The eight softmax warps are two: the halves of the columns."""
+    m = Model()
+    for name, count in dict(a_full=1, a_empty=2, s_full=1, s_free=2, dp_full=1, p_ready=2, ds_ready=2, o_full=1, o_free=2, row_sum=2).items():
+        m.barrier(name, count)
+    for i in range(ring):
+        m.barrier(("full", i), 1)
+        m.barrier(("empty", i), 1)
+    tiles = [(ic, t, t == n - 1) for ic, n in enumerate(items) for t in range(n)]
+
+    def full(wait, load):
+        wait(("full", load % ring), load // ring)
+
+    for x in range(2):
+        wait, arrive, write, read = m.warp(f"softmax {x}")
+        for g, (ic, t, last) in enumerate(tiles):
+            n0, n1 = 2 * g, 2 * g + 1
+            wait("s_full", g)
+            if keys:
+                full(wait, n0)
+            read("S", g)
+            arrive("s_free")
+            wait("dp_full", g)
+            if keys:
+                full(wait, n1)
+            read("dP", g)
+            write(("P", x), g)
+            arrive("p_ready")
+            write(("dS", x), g)
+            arrive("ds_ready")
+            if not last:
+                continue
+            if not keys:
+                if ordered_sums and ic > 0:
+                    wait("o_free", ic - 1)
+                write(("sums", x), ic)
+                arrive("row_sum")
+                wait("row_sum", ic)
+                read(("sums", 1 - x), ic)
+            wait("o_full", ic)
+            read("sum of P", ic)
+            read("sum of dS", ic)
+            arrive("o_free")
+
+    wait, arrive, write, read = m.warp("scores")
+    for g, (ic, t, last) in enumerate(tiles):
+        if t == 0:
+            wait("a_full", ic)
+        full(wait, 2 * g)
+        if ordered and t > 0:
+            wait("dp_full", g - 1)
+        if g > 0:
+            wait("s_free", g - 1)
+        read("A", ic)
+        read(("ring", 2 * g % ring), 2 * g)
+        write("S", g)
+        arrive("s_full")
+        if last:
+            arrive("a_empty")
+
+    wait, arrive, write, read = m.warp("sums")
+    for g, (ic, t, last) in enumerate(tiles):
+        n0, n1 = 2 * g, 2 * g + 1
+        if t == 0:
+            wait("a_full", ic)
+        if ordered and t > 0:
+            wait("s_full", g)
+        full(wait, n1)
+        read("A", ic)
+        read(("ring", n1 % ring), n1)
+        write("dP", g)
+        arrive("dp_full")
+        if not keys:
+            arrive(("empty", n1 % ring))
+        if last:
+            arrive("a_empty")
+        wait("p_ready", g)
+        if t == 0 and ic > 0:
+            wait("o_free", ic - 1)
+        n = n1 if keys else n0
+        read(("ring", n % ring), n)
+        for x in range(2):
+            read(("P", x), g)
+        write("sum of P", ic)
+        if keys:
+            arrive(("empty", n1 % ring))
+        wait("ds_ready", g)
+        for x in range(2):
+            read(("dS", x), g)
+        read(("ring", n0 % ring), n0)
+        write("sum of dS", ic)
+        arrive(("empty", n0 % ring))
+        if last:
+            arrive("o_full")
+
+    wait, arrive, write, read = m.warp("resident tiles")
+    for ic in range(len(items)):
+        if ic > 0:
+            wait("a_empty", ic - 1)
+        write("A", ic)
+        arrive("a_full")
+    wait, arrive, write, read = m.warp("ring")
+    for n in range(2 * len(tiles)):
+        if n >= ring:
+            wait(("empty", n % ring), n // ring - 1)
+        write(("ring", n % ring), n)
+        arrive(("full", n % ring))
+    return m
+
+
+ITEMS = [(1, 1, 1, 1), (1, 2, 1, 3, 1), (3, 1, 1, 2), (5, 4)]
+# (rows of a tile are 128 with rings of 5 and 8 tiles, or 64 with 5 and 3)
+SHAPES = [(True, 5), (True, 8), (False, 5), (False, 3)]
+
+
+@pytest.mark.parametrize("ordered,ring", SHAPES)
+@pytest.mark.parametrize("items", ITEMS)
+@pytest.mark.parametrize("keys", [False, True])
+def test_dense_modes(items, keys, ordered, ring):
+    backward(items, keys, ordered, ring).check()
+
+
+@pytest.mark.parametrize("ordered,ring", SHAPES)
+def test_row_sums_of_an_item_of_one_tile_wait_for_the_reads_of_the_item_before(ordered, ring):
+    with pytest.raises(Fault, match="sums"):
+        backward((1, 1, 1, 1), False, ordered, ring, ordered_sums=False).check()
+    backward((2, 2, 2), False, ordered, ring, ordered_sums=False).check()       # (the sum of the first tile's P orders the second's dP)
