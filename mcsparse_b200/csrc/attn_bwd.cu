@@ -265,7 +265,7 @@ __global__ void __launch_bounds__(threads_of(kMode), 1) attn_bwd_kernel(const At
   };
 
   if (tid == 0) {
-    for (int i = 0; i < R; ++i) { mbar_init(bar(L::kFull + i), kGather ? TN : 1); mbar_init(bar(L::kEmpty + i), 1); }
+    for (int i = 0; i < R; ++i) { mbar_init(bar(L::kFull + i), kGather ? TN + kGatherWarps : 1); mbar_init(bar(L::kEmpty + i), 1); }
     mbar_init(bar(L::kAFull), kGather ? 256 : 1);
     mbar_init(bar(L::kAEmpty), 2);
     mbar_init(bar(L::kSFull), 1);
@@ -670,6 +670,10 @@ __global__ void __launch_bounds__(threads_of(kMode), 1) attn_bwd_kernel(const At
             }
             batch = batch == kWarps - 1 ? 0 : batch + 1;
           }
+          // Every warp has a part in every load, with rows of it or without: a load that could be consumed without this warp might free its
+          // slot again before the wait above has seen the phase that it waits for, whose parity would then never come back.
+          __syncwarp();
+          if (lane == 0) mbar_arrive(bar(L::kFull + slot));
         }
         if (!ok) break;
         if (t == it.t0) {

@@ -71,19 +71,30 @@ class Model:
                 self.run(name, at)
 
 
-def backward(items, keys, ordered, ring, ordered_sums=True):
+def backward(items, keys, ordered, ring, gather=False, ordered_sums=True, all_arrive=True):
     """One CTA of attn_bwd_kernel that walks `items` (tiles of each).  `keys`: the mode of dK and dV, else that of dQ.  `ordered`: tiles of 128
-    rows, whose S and dP are issued in a fixed order.  The eight softmax warps are two: the halves of the columns."""
+    rows, whose S and dP are issued in a fixed order.  `gather`: six warps copy batches of 32 rows in turn, instead of two that issue TMA.
+    The eight softmax warps are two: the halves of the columns."""
     m = Model()
-    for name, count in dict(a_full=1, a_empty=2, s_full=1, s_free=2, dp_full=1, p_ready=2, ds_ready=2, o_full=1, o_free=2, row_sum=2).items():
+    batches = (4 if ordered else 2) if gather else 1
+    res_batches = 8 if gather else 1
+    for name, count in dict(a_full=res_batches, a_empty=2, s_full=1, s_free=2, dp_full=1, p_ready=2, ds_ready=2, o_full=1, o_free=2, row_sum=2).items():
         m.barrier(name, count)
     for i in range(ring):
-        m.barrier(("full", i), 1)
+        m.barrier(("full", i), batches + (GATHER_WARPS if gather and all_arrive else 0))
         m.barrier(("empty", i), 1)
     tiles = [(ic, t, t == n - 1) for ic, n in enumerate(items) for t in range(n)]
 
     def full(wait, load):
         wait(("full", load % ring), load // ring)
+
+    def read_tile(read, load):
+        for q in range(batches):
+            read(("ring", load % ring, q), load)
+
+    def read_resident(read, ic):
+        for q in range(res_batches):
+            read(("A", q), ic)
 
     for x in range(2):
         wait, arrive, write, read = m.warp(f"softmax {x}")
@@ -94,12 +105,16 @@ def backward(items, keys, ordered, ring, ordered_sums=True):
                 full(wait, n0)
             read("S", g)
             arrive("s_free")
+            if keys:
+                read(("statistics", n0 % ring), n0)
             wait("dp_full", g)
             if keys:
                 full(wait, n1)
             read("dP", g)
             write(("P", x), g)
             arrive("p_ready")
+            if keys:
+                read(("statistics", n1 % ring), n1)
             write(("dS", x), g)
             arrive("ds_ready")
             if not last:
@@ -125,8 +140,8 @@ def backward(items, keys, ordered, ring, ordered_sums=True):
             wait("dp_full", g - 1)
         if g > 0:
             wait("s_free", g - 1)
-        read("A", ic)
-        read(("ring", 2 * g % ring), 2 * g)
+        read_resident(read, ic)
+        read_tile(read, 2 * g)
         write("S", g)
         arrive("s_full")
         if last:
@@ -140,8 +155,8 @@ def backward(items, keys, ordered, ring, ordered_sums=True):
         if ordered and t > 0:
             wait("s_full", g)
         full(wait, n1)
-        read("A", ic)
-        read(("ring", n1 % ring), n1)
+        read_resident(read, ic)
+        read_tile(read, n1)
         write("dP", g)
         arrive("dp_full")
         if not keys:
@@ -152,36 +167,64 @@ def backward(items, keys, ordered, ring, ordered_sums=True):
         if t == 0 and ic > 0:
             wait("o_free", ic - 1)
         n = n1 if keys else n0
-        read(("ring", n % ring), n)
+        read_tile(read, n)
         for x in range(2):
             read(("P", x), g)
         write("sum of P", ic)
         if keys:
+            # (the deltas of this slot may still be wanted; the ring is loaded in order, and T0's slot comes first)
             arrive(("empty", n1 % ring))
         wait("ds_ready", g)
         for x in range(2):
             read(("dS", x), g)
-        read(("ring", n0 % ring), n0)
+        read_tile(read, n0)
         write("sum of dS", ic)
         arrive(("empty", n0 % ring))
         if last:
             arrive("o_full")
 
+    if gather:
+        for w in range(GATHER_WARPS):
+            wait, arrive, write, read = m.warp(f"rows {w}")
+            n = batch = 0
+            for ic, t, last in tiles:
+                for n in (n, n + 1):
+                    if n >= ring:
+                        wait(("empty", n % ring), n // ring - 1)
+                    for q in range(batches):
+                        if batch % GATHER_WARPS == w:
+                            write(("ring", n % ring, q), n)
+                            arrive(("full", n % ring))
+                        batch += 1
+                    if all_arrive:
+                        arrive(("full", n % ring))
+                n += 1
+                if t == 0:
+                    if ic > 0:
+                        wait("a_empty", ic - 1)
+                    for q in range(res_batches):
+                        if batch % GATHER_WARPS == w:
+                            write(("A", q), ic)
+                            arrive("a_full")
+                        batch += 1
+        return m
     wait, arrive, write, read = m.warp("resident tiles")
     for ic in range(len(items)):
         if ic > 0:
             wait("a_empty", ic - 1)
-        write("A", ic)
+        write(("A", 0), ic)
         arrive("a_full")
     wait, arrive, write, read = m.warp("ring")
     for n in range(2 * len(tiles)):
         if n >= ring:
             wait(("empty", n % ring), n // ring - 1)
-        write(("ring", n % ring), n)
+        write(("ring", n % ring, 0), n)
+        write(("statistics", n % ring), n)
         arrive(("full", n % ring))
     return m
 
 
+GATHER_WARPS = 6
 ITEMS = [(1, 1, 1, 1), (1, 2, 1, 3, 1), (3, 1, 1, 2), (5, 4)]
 # (rows of a tile are 128 with rings of 5 and 8 tiles, or 64 with 5 and 3)
 SHAPES = [(True, 5), (True, 8), (False, 5), (False, 3)]
@@ -199,3 +242,17 @@ def test_row_sums_of_an_item_of_one_tile_wait_for_the_reads_of_the_item_before(o
     with pytest.raises(Fault, match="sums"):
         backward((1, 1, 1, 1), False, ordered, ring, ordered_sums=False).check()
     backward((2, 2, 2), False, ordered, ring, ordered_sums=False).check()       # (the sum of the first tile's P orders the second's dP)
+
+
+@pytest.mark.parametrize("ordered,ring", SHAPES)
+@pytest.mark.parametrize("items", [*ITEMS, (4, 1, 1, 5), (7, 1, 3)])
+def test_gathered_keys(items, ordered, ring):
+    backward(items, False, ordered, ring, gather=True).check()
+
+
+@pytest.mark.parametrize("ordered,ring", SHAPES)
+def test_a_warp_without_rows_of_a_load_has_a_part_in_it_all_the_same(ordered, ring):
+    """Without its arrival the load is consumed, and the slot's barrier moves on, before the warp has seen the phase that it waits for."""
+    with pytest.raises(Fault, match="stuck"):
+        for items in ((4, 1, 1, 5), (7, 1, 3), (1, 1, 1, 1, 1, 1, 1)):
+            backward(items, False, ordered, ring, gather=True, all_arrive=False).check()
