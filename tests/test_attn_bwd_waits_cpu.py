@@ -1,11 +1,11 @@
-"""The waits of the attention's backward kernel (csrc/attn_bwd.cu), modelled on the CPU.
+"""The waits of the attention's backward kernels (csrc/attn_bwd.cu, csrc/attn_bwd_gather.cu), modelled on the CPU.
 
 Every warp, or group of warps with one role, is a list of steps: wait for a phase of a barrier, arrive at one, write a place, read a place
 and find what was meant for it.  Barriers behave as the hardware's: a wait sees the parity of the running phase only, so a barrier that has
 moved two phases on looks as if it had not moved.  A run holds one warp up in front of one of its steps until nobody else can go on, then
 lets it go; every step of every warp is held up once.  No run may get stuck or read what was not meant for the reader.
 
-The model follows the kernel's program order by hand.  Each of its switches takes one of the kernel's waits away, and the model has to find
+The models follow the kernels' program order by hand.  Each switch takes one of the kernel's waits away, and the model has to find
 what that wait is for.
 """
 
@@ -256,3 +256,106 @@ def test_a_warp_without_rows_of_a_load_has_a_part_in_it_all_the_same(ordered, ri
     with pytest.raises(Fault, match="stuck"):
         for items in ((4, 1, 1, 5), (7, 1, 3), (1, 1, 1, 1, 1, 1, 1)):
             backward(items, False, ordered, ring, gather=True, all_arrive=False).check()
+
+
+def contributions(items, blocks, ring):
+    """One CTA of attn_bwd_gather_dkv_kernel that walks groups of `items` tiles, `blocks` column blocks of 128: softmax warps by halves of the
+    columns, the issuer, three warps that copy rows, the warps that copy out as one."""
+    m = Model()
+    for name, count in dict(a_full=8, a_empty=1, s_full=1, dp_full=1, p_ready=2, ds_ready=2, dv_full=1, dv_free=1, dk_full=1, dk_free=1).items():
+        m.barrier(name, count)
+    for i in range(ring):
+        m.barrier(("full", i), 4)
+        m.barrier(("empty", i), 1)
+    tiles = [(ic, t, t == n - 1) for ic, n in enumerate(items) for t in range(n)]
+
+    for x in range(2):
+        wait, arrive, write, read = m.warp(f"softmax {x}")
+        for g, (ic, t, last) in enumerate(tiles):
+            if t == 0:
+                wait("a_full", ic)
+            wait("s_full", g)
+            read(("S", x), g)
+            read(("A", 0), ic)                               # statistics come with the first rows
+            write(("S", x), ("P", g))
+            arrive("p_ready")
+            wait("dp_full", g)
+            read(("dP", x), g)
+            read(("A", 4), ic)
+            write(("dP", x), ("dS", g))
+            arrive("ds_ready")
+
+    wait, arrive, write, read = m.warp("issuer")
+    n = block = 0
+    for g, (ic, t, last) in enumerate(tiles):
+        if t == 0:
+            wait("a_full", ic)
+        for name, done in (("S", "s_full"), ("dP", "dp_full")):
+            for cb in range(blocks):
+                wait(("full", n % ring), n // ring)
+                for q in range(4):
+                    read(("ring", n % ring, q), n)
+                for q in range(8):
+                    read(("A", q), ic)
+                for x in range(2):
+                    write((name, x), g)
+                arrive(("empty", n % ring))
+                n += 1
+            arrive(done)
+        wait("p_ready", g)
+        for cb in range(blocks):
+            if block > 0:
+                wait("dv_free", block - 1)
+            for x in range(2):
+                read(("S", x), ("P", g))
+            for q in range(8):
+                read(("A", q), ic)
+            write("dV", block)
+            arrive("dv_full")
+            if cb == 0:
+                wait("ds_ready", g)
+            if block > 0:
+                wait("dk_free", block - 1)
+            for x in range(2):
+                read(("dP", x), ("dS", g))
+            write("dK", block)
+            arrive("dk_full")
+            block += 1
+        if last:
+            arrive("a_empty")
+
+    for w in range(3):
+        wait, arrive, write, read = m.warp(f"rows {w}")
+        n = batch = 0
+        for ic, t, last in tiles:
+            for e in range(2 * blocks):
+                if n >= ring:
+                    wait(("empty", n % ring), n // ring - 1)
+                for q in range(4):
+                    if batch % 3 == w:
+                        write(("ring", n % ring, q), n)
+                        arrive(("full", n % ring))
+                    batch += 1
+                if t == 0 and e == 0:
+                    if ic > 0:
+                        wait("a_empty", ic - 1)
+                    for q in range(8):
+                        if batch % 3 == w:
+                            write(("A", q), ic)
+                            arrive("a_full")
+                        batch += 1
+                n += 1
+
+    wait, arrive, write, read = m.warp("copy out")
+    for block in range(len(tiles) * blocks):
+        for name, full, free in (("dV", "dv_full", "dv_free"), ("dK", "dk_full", "dk_free")):
+            wait(full, block)
+            read(name, block)
+            arrive(free)
+    return m
+
+
+@pytest.mark.parametrize("blocks,ring", [(1, 8), (1, 4), (2, 2)])
+@pytest.mark.parametrize("items", [*ITEMS, (4, 1, 1, 5)])
+def test_contributions_of_gathered_keys(items, blocks, ring):
+    contributions(items, blocks, ring).check()
