@@ -247,8 +247,8 @@ int64_t mcs_dense_attn_bwd_workspace_bytes(const mcs_attn_bwd_args* args);
  * Backward pass of the gather-KV attention (mcs_gather_attn_fwd without residual): the same gradients with the key multiset of
  * each query group, through perm as in the forward pass (out, dout, lse and dq are in the original row order).  A key's dk and
  * dv sum over the groups that selected it, once per entry; keys that none selected get zeros.  Indices outside [0, Sk) are
- * clamped, as in the forward pass; positions whose entry of perm is outside [0, Sq) take no part.  Sums in a fixed order:
- * bit-equal from run to run.  k, v, q, dout may have any 16-byte aligned strides.  The workspace holds fp32 contributions of up to 4 GiB, or of one head
+ * clamped, as in the forward pass; positions whose entry of perm is outside [0, Sq) take no part, and rows of dq that no entry of
+ * perm names are zero.  Sums in a fixed order: bit-equal from run to run.  k, v, q, dout may have any 16-byte aligned strides.  The workspace holds fp32 contributions of up to 4 GiB, or of one head
  * (8 * D * M * gather_len bytes) where that is more.
  */
 int mcs_gather_attn_bwd(const mcs_attn_bwd_args* args, void* stream);

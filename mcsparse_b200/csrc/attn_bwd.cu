@@ -24,7 +24,8 @@ constexpr int kMaxSmem = 232448;
 // Sixteen lanes per row, four rows at a time: neg_delta = -sum(dout * out) and neg_lse2 of every tile row (memory-bound: dout and out
 // are read once, eight 16-byte loads of a thread in flight), and for fp16 the largest norms of rows of dout and of v.  Only rows that take
 // part in finite results count for these: rows with an infinity or NaN give no finite dS whatever its scale, and rows of v that no group
-// selected (key_start, gathered keys only) may hold anything.
+// selected (key_start, gathered keys only) may hold anything.  With perm dQ is zeroed on the way: its rows are written through perm, whose
+// entries may be out of range.
 template <bool kFp16>
 __device__ __forceinline__ float dot8(uint4 a, uint4 b, float acc) {
   const uint32_t x[4] = {a.x, a.y, a.z, a.w}, y[4] = {b.x, b.y, b.z, b.w};
@@ -49,6 +50,7 @@ __global__ void __launch_bounds__(256) attn_bwd_stats_kernel(const AttnBwdParams
   const int chunks = p.D / 8;
   const uint8_t* gb = reinterpret_cast<const uint8_t*>(p.dout) + 2 * ((size_t)b * p.dout_stride[0] + (size_t)h * p.dout_stride[2]);
   const uint8_t* ob = reinterpret_cast<const uint8_t*>(p.out) + 2 * ((size_t)b * p.out_stride[0] + (size_t)h * p.out_stride[2]);
+  uint8_t* qb = reinterpret_cast<uint8_t*>(p.dq) + 2 * ((size_t)b * p.dq_stride[0] + (size_t)h * p.dq_stride[2]);
   float m_do = 0.f, m_v = 0.f;
   // fp16: every second CTA takes rows of v instead
   const int share = kFp16 ? 2 : 1, blk = blockIdx.x / share, step = gridDim.x / share;
@@ -61,6 +63,15 @@ __global__ void __launch_bounds__(256) attn_bwd_stats_kernel(const AttnBwdParams
       const int i = base + u * 16 + sub, r = i & 127, pos = (i >> 7) * p.group_rows + r;
       row[u] = -1;
       if (i < rows && r < p.group_rows && pos < p.Sq) row[u] = query_row(p, bh, pos);
+    }
+    if (p.perm != nullptr) {
+      // dQ's rows are written through perm: those that no entry of it names have no gradient
+#pragma unroll
+      for (int u = 0; u < kRows; ++u) {
+        const int i = base + u * 16 + sub, r = i & 127, pos = (i >> 7) * p.group_rows + r;
+        if (i >= rows || r >= p.group_rows || pos >= p.Sq) continue;
+        for (int c = l16; c < chunks; c += 16) *reinterpret_cast<uint4*>(qb + 2 * (size_t)pos * p.dq_stride[1] + c * 16) = make_uint4(0, 0, 0, 0);
+      }
     }
     for (int c = l16; c < chunks; c += 16) {
       uint4 x[kRows], y[kRows];

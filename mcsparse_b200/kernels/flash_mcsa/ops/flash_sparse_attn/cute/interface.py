@@ -474,7 +474,7 @@ def flash_attn_gather_kv_backward_func(
     with ``return_lse=True`` (a residual is added outside and gets ``dout`` itself as its gradient, in permuted order where
     ``perm`` is given).  Layouts, indices (int32 or :class:`PackedIndices`), lengths, ``perm`` and ``group_rows`` as in the
     forward pass; all gradients are in the original row order.  A key's gradient sums over the groups that selected it, once
-    per entry; keys that no group selected get zeros.  Sums are fp32 in a fixed order: the same inputs give the same bits.
+    per entry; keys that no group selected get zeros, as do rows of dq that no entry of ``perm`` names.  Sums are fp32 in a fixed order: the same inputs give the same bits.
 
     The contributions of up to 4 GiB at a time (at least one head's: 8 * D bytes per entry) pass through a temporary buffer.
     (The reference is forward-only.)

@@ -46,3 +46,31 @@ def test_gathered_lists_of_few_tiles(cuda_device, D, most, dtype):
     for _ in range(REPEATS):
         again = flash_attn_gather_kv_backward_func(dout, q, k, v, out, lse, gi, **kw)
         assert all(torch.equal(a, b) for a, b in zip(first, again))
+
+
+@pytest.mark.parametrize("D,dtype", [(64, torch.bfloat16), (96, torch.float16), (144, torch.bfloat16)])
+def test_rows_of_dq_that_perm_does_not_name_are_zero(cuda_device, D, dtype):
+    """Entries of perm out of range, and a row named twice: the rows left over have no gradient, whatever their memory held."""
+    from mcsparse_b200.kernels.flash_mcsa.ops import attn_bwd
+    g = torch.Generator(device=cuda_device).manual_seed(D)
+    B, H, S = 2, 2, 300
+    q, k, v, dout = (torch.randn(B, S, H, D, generator=g, device=cuda_device).to(dtype) for _ in range(4))
+    gi = torch.rand(B, H, 3, S, generator=g, device=cuda_device).argsort(dim=-1)[..., :128].int().contiguous()
+    perm = torch.stack([torch.randperm(S, generator=g, device=cuda_device) for _ in range(B * H)])
+    out, lse = flash_attn_gather_kv_func(q, k, v, gi, return_lse=True, perm=perm)
+    want = flash_attn_gather_kv_backward_func(dout, q, k, v, out, lse, gi, perm=perm)
+    left = perm[:, [5, 140, 299]].clone()
+    bad = perm.clone()
+    bad[:, 5], bad[:, 140], bad[:, 299] = S, -1, perm[:, 298]
+    big = torch.full((B, S + 2, H + 2, D + 16), float("nan"), dtype=dtype, device=cuda_device)
+    dq = big[:, 1:-1, 1:-1, 8:D + 8]
+    attn_bwd.launch_backward("mcs_gather_attn_bwd", dout, q, k, v, out, lse, dq, torch.empty_like(k), torch.empty_like(v), D ** -0.5, gi, None, bad)
+    for bh in range(B * H):
+        b, h = divmod(bh, H)
+        assert bool((dq[b, left[bh], h] == 0).all())
+        others = torch.ones(S, dtype=torch.bool, device=cuda_device)
+        others[left[bh]] = False
+        others[perm[bh, 298]] = False                        # (named twice)
+        assert torch.equal(dq[b, others, h], want[0][b, others, h])
+    dq.fill_(float("nan"))
+    assert bool(big.isnan().all())                           # nothing beside the rows was written
