@@ -852,11 +852,13 @@ struct Plan { bool pair_k, pair_q; int stat_rows, dq_splits, kv_splits, segs, he
 constexpr size_t kAlign = 256;
 size_t up(size_t n) { return (n + kAlign - 1) / kAlign * kAlign; }
 
-// Whether tiles of a streamed axis of S rows hold their rows twice: up to 64 rows, where that fills padding (D <= 128), and up to 256
-// where the tiles, now twice as many, are no more than the SMs, most of which would be idle.  Errors of dK relative to the result's own
-// rounding, 65 to 130 queries on 33 to 90 keys: 1.51 to 1.56 without, 1.00 with it.  Time of a captured call of 128 x 128 x 128: 17.9 and 21.6 us;
-// of 4 heads x 512 x 512 x 128 26.2 and 33.7, for sums over which the rounding averages out (1.4): not taken there.
-bool pick_paired(long long items, int S, int TN) { return S <= 64 || (S <= 256 && items * ((S + TN / 2 - 1) / (TN / 2)) <= 148); }
+// Whether tiles of a streamed axis of S rows hold their rows twice: up to 64 rows, where that fills padding (D <= 128), and where the tiles of
+// all items, now twice as many, are no more than the SMs, most of which would be idle: there accuracy takes time from nobody else.  Errors
+// relative to those of a 32-bit computation that rounds its results once, 1 to 8 heads, 130 to 2,000 rows on 7 to 2,000, D 64 to 144: single
+// parts about 1.4 whatever the length, up to 1.9 where few rows carry the sum, and 88 of 1,632 calls above 1.5; with this rule 1.0 where it takes
+// two parts, and 2 calls above 1.5 (1.52).  Time of a captured call in bf16, D = 128: 128 x 128 17.9 -> 21.6 us, 2 heads x 300 x 300
+// 26.7 -> 34.5, 4 heads x 512 x 512 29.0 -> 37.0, 1,000 x 1,000 37.0 -> 39.3, 2,000 x 300 34.9 -> 44.4.
+bool pick_paired(long long items, int S, int TN) { return S <= 64 || items * ((S + TN / 2 - 1) / (TN / 2)) <= 148; }
 
 // Rows of a streamed tile: as many as tensor memory holds beside both sums, and shared memory beside the resident tiles.  (96 rows up to
 // D = 160 would fit, with a ring of three tiles instead of five: 18,944 x 144 took 488 us a side against 455.)

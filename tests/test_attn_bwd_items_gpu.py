@@ -74,3 +74,19 @@ def test_rows_of_dq_that_perm_does_not_name_are_zero(cuda_device, D, dtype):
         assert torch.equal(dq[b, others, h], want[0][b, others, h])
     dq.fill_(float("nan"))
     assert bool(big.isnan().all())                           # nothing beside the rows was written
+
+
+@pytest.mark.parametrize("D,dtype", [(128, torch.bfloat16), (64, torch.float16), (144, torch.bfloat16)])
+def test_dq_of_full_lists_has_the_dense_bits(cuda_device, D, dtype):
+    """Every group lists every key in order, and the dense call neither splits the keys nor takes its operands in two parts: the same products
+    in the same order."""
+    g = torch.Generator(device=cuda_device).manual_seed(D)
+    B, H, Sq, Sk = 1, 12, 1500, 512
+    mk = lambda L: torch.randn(B, L, H, D, generator=g, device=cuda_device).to(dtype)
+    q, k, v, dout = mk(Sq), mk(Sk), mk(Sk), mk(Sq)
+    gi = torch.arange(Sk, device=cuda_device, dtype=torch.int32).expand(B, H, 12, Sk).contiguous()
+    heads = lambda x: x.transpose(1, 2)
+    out, lse = full_attention_with_lse(heads(q), heads(k), heads(v))
+    dense = full_attention_backward(heads(dout), heads(q), heads(k), heads(v), out, lse)
+    got = flash_attn_gather_kv_backward_func(dout, q, k, v, heads(out), lse, gi)
+    assert torch.equal(heads(dense[0]), got[0])
