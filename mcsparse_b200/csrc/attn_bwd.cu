@@ -997,7 +997,7 @@ int launch_type(AttnBwdParams& p, const Plan& w, bool gather, cudaStream_t strea
 
 }  // namespace
 
-int64_t attn_bwd_workspace_bytes(const AttnBwdParams& p, bool gather, bool) { return (int64_t)make_plan(p, gather).total; }
+int64_t attn_bwd_workspace_bytes(const AttnBwdParams& p, bool gather) { return (int64_t)make_plan(p, gather).total; }
 
 int launch_attn_bwd(AttnBwdParams& p, bool gather, bool fp16, void* workspace, cudaStream_t stream) {
   const Plan w = make_plan(p, gather);

@@ -392,7 +392,7 @@ static int attn_bwd_params(const mcs_attn_bwd_args* a, bool gather, mcs::AttnBwd
   if (gather && tiles * a->gather_len > 0x7fffffffLL) return MCS_ERR_TOO_LARGE;       // rows of one head's entries are 32-bit
   p.B = a->B; p.H = a->H; p.Sq = a->Sq; p.Sk = a->Sk; p.D = a->D;
   p.gather_len = a->gather_len; p.group_rows = (int)rows; p.M = (int)tiles;
-  p.scale = a->softmax_scale; p.scale_log2 = a->softmax_scale * 1.4426950408889634f;
+  p.scale_log2 = a->softmax_scale * 1.4426950408889634f;
   // softmax over a single key does not depend on the scores
   p.out_scale = (!gather && a->Sk == 1) ? 0.f : a->softmax_scale;
   p.splits = 1;
@@ -415,7 +415,7 @@ static int attn_bwd_dispatch(const mcs_attn_bwd_args* a, bool gather, void* stre
   }
   if (reinterpret_cast<uintptr_t>(a->workspace) % 256) return MCS_ERR_BAD_ALIGNMENT;
   const bool fp16 = a->dtype == MCS_DTYPE_FP16;
-  if (mcs::attn_bwd_workspace_bytes(p, gather, fp16) > a->workspace_bytes) return MCS_ERR_WORKSPACE_TOO_SMALL;
+  if (mcs::attn_bwd_workspace_bytes(p, gather) > a->workspace_bytes) return MCS_ERR_WORKSPACE_TOO_SMALL;
   p.q = a->q; p.k = a->k; p.v = a->v; p.out = a->out; p.dout = a->dout; p.lse = a->lse;
   p.dq = a->dq; p.dk = a->dk; p.dv = a->dv;
   p.gi = a->gi; p.gl = a->gl; p.perm = a->perm; p.status = a->status;
@@ -431,7 +431,7 @@ int mcs_dense_attn_bwd(const mcs_attn_bwd_args* a, void* stream) { return attn_b
 int64_t mcs_dense_attn_bwd_workspace_bytes(const mcs_attn_bwd_args* a) {
   mcs::AttnBwdParams p{};
   const int rc = attn_bwd_params(a, false, p);
-  return rc != 0 ? rc : mcs::attn_bwd_workspace_bytes(p, false, a->dtype == MCS_DTYPE_FP16);
+  return rc != 0 ? rc : mcs::attn_bwd_workspace_bytes(p, false);
 }
 
 int mcs_gather_attn_bwd(const mcs_attn_bwd_args* a, void* stream) { return attn_bwd_dispatch(a, true, stream); }
@@ -439,7 +439,7 @@ int mcs_gather_attn_bwd(const mcs_attn_bwd_args* a, void* stream) { return attn_
 int64_t mcs_gather_attn_bwd_workspace_bytes(const mcs_attn_bwd_args* a) {
   mcs::AttnBwdParams p{};
   const int rc = attn_bwd_params(a, true, p);
-  return rc != 0 ? rc : mcs::attn_bwd_workspace_bytes(p, true, a->dtype == MCS_DTYPE_FP16);
+  return rc != 0 ? rc : mcs::attn_bwd_workspace_bytes(p, true);
 }
 
 int mcs_rotary(const mcs_rotary_args* a, void* stream) {

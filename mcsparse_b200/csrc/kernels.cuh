@@ -182,7 +182,7 @@ struct AttnBwdParams {
   int64_t q_stride[3], k_stride[3], v_stride[3], out_stride[3], dout_stride[3], dq_stride[3], dk_stride[3], dv_stride[3];
   int B, H, Sq, Sk, D;
   int gather_len, group_rows, M;              // M query tiles of up to 128 rows (group_rows of them used)
-  float scale, scale_log2;                    // softmax scale; times log2(e)
+  float scale_log2;                           // softmax scale times log2(e)
   float out_scale;                            // factor of dq and dk: the scale, or 0 where a single key leaves no gradient
   // workspace
   int stat_rows;                              // rows per head of the next three, at least 128 M
@@ -197,7 +197,7 @@ struct AttnBwdParams {
   int32_t *entry_row, *key_start, *seg_count, *block_sum;
   int bh0, bh_count;                          // heads of this launch
 };
-int64_t attn_bwd_workspace_bytes(const AttnBwdParams& p, bool gather, bool fp16);
+int64_t attn_bwd_workspace_bytes(const AttnBwdParams& p, bool gather);
 int launch_attn_bwd_gather_rows(const AttnBwdParams& p, int segs, cudaStream_t stream);
 int launch_attn_bwd_gather_dkv(AttnBwdParams& p, bool fp16, int heads_per_pass, cudaStream_t stream);
 int launch_attn_bwd(AttnBwdParams& p, bool gather, bool fp16, void* workspace, cudaStream_t stream);
