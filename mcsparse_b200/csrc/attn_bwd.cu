@@ -179,7 +179,7 @@ __global__ void __launch_bounds__(256) attn_bwd_stats_kernel(const AttnBwdParams
 // the tensor pipe as long as the kernel of dK and dV does.  The sum of dS before rounding, too, is taken: it is what delta is off
 // by, and the key side, which runs second, gets delta without it (dK: 2.7e-3 -> 2.4e-3 with lists of selected keys).
 //
-// Short sums (kPaired; see pick_paired): the rounding of P and dS does not average out over a few rows, and
+// Short sums, and others on idle SMs (kPaired; see pick_paired): the rounding of P and dS does not average out over a few rows, and
 // where these resemble one another (neighbouring tokens) the sums cancel and the rounding does not: 7 queries on 33 keys x 64, bf16: error of dK
 // 3.5e-3 of its norm, 1.6e-3 of it the result's own rounding.  A tile then holds TN / 2 rows twice, and the second half of the softmax
 // threads stores what the first half's rounding left, so that the sums take P and dS with twice the bits.  Up to TN / 2 rows this fills
@@ -207,8 +207,8 @@ constexpr bool fits = SmemB<DB, TN>::kDynamic <= kMaxSmem && SmemB<DB, TN>::kCol
 static_assert(fits<1, 128> && fits<2, 128> && fits<3, 64> && fits<4, 64>, "227 KB of shared memory, 512 columns of tensor memory");
 
 // Warps: eight softmax warps, two issuers, then for the dense modes the producers of the resident tiles and of the ring, for gathered keys
-// six warps that copy both: 512 threads of 128 registers.  (24 heads x 256 groups x 2,048 keys x 128: three warps, which leave 168
-// registers, 1.63 ms, four 1.54, seven 1.48.)
+// six warps that copy both: 512 threads of 128 registers (about 200 bytes of spills per thread at D <= 128).  24 heads x 256 groups x 2,048 keys
+// x 128: 1.39 ms.  With one issuing warp instead of two, three copying warps, which leave 168 registers, took 1.63 ms, four 1.54, seven 1.48.
 constexpr int kIssueWarp = 8, kScoreWarp = 9, kLoadWarp0 = 10, kGatherWarps = 6;
 constexpr int threads_of(int mode) { return mode == kDqGather ? 32 * (kLoadWarp0 + kGatherWarps) : 384; }
 
@@ -548,7 +548,7 @@ __global__ void __launch_bounds__(threads_of(kMode), 1) attn_bwd_kernel(const At
       tc_fence_after();
     };
     // (unrolled, the k-steps of padding predicated off: with a rolled loop of kd steps one of the products had its last step
-    // accumulated nine times)
+    // accumulated nine times; why is not known)
     auto scores = [&](uint32_t d, uint32_t a_tile, int load) {
       const uint32_t alo = lo_kmajor(a_tile), blo = lo_kmajor(sRing(load % R));
       auto step = [&](int j) {
@@ -843,8 +843,8 @@ int pick_splits(long long items, int T, double tile_us, double part_bytes) {
   return pick;
 }
 
-// Most bytes of one pass's contributions in the gather call (a single head's may be more).  They pass through DRAM anyway; smaller
-// passes would only add launches with a partly filled last wave.
+// Most bytes of one pass's contributions in the gather call (a single head's may be more).  24 heads x 256 groups x 2,048 keys x 128, whole call:
+// 7.41 ms in passes of 4 GiB, 7.44 in 2, 7.73 in 1 (more launches with a partly filled last wave).
 constexpr size_t kPartsBytes = 4ull << 30;
 
 struct Plan { bool pair_k, pair_q; int stat_rows, dq_splits, kv_splits, segs, heads_per_pass; size_t stats, row_max, entries, starts, counts, blocks, parts, total; };

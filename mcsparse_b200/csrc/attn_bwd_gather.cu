@@ -4,8 +4,7 @@
 // places, so the sums cannot stay in tensor memory as in the dense call: a group's 128 x D contributions to a tile of 128 gathered keys
 // go to rows of an fp32 buffer, and a second kernel adds the rows of every key.  The buffer is laid out by key: the entries
 // (group, slot) that name key j take consecutive rows, in the order of groups, so that the second kernel reads it once, in
-// order, and the sums (and their bits) do not depend on which CTA came first.  (Adding with atomics in place would move the same bytes
-// through L2 and leave the order to chance.)  Equal entries inside one group have equal contributions, so their order does not matter.
+// order, and the sums (and their bits) do not depend on which CTA came first, which with atomics in place would be left to chance.  Equal entries inside one group have equal contributions, so their order does not matter.
 //
 // Bound: the buffer is written and read once, 8 D bytes per entry either way (12.9 GB + 12.9 GB at 24 heads x 256 groups x 2,048
 // keys x 128: 3.9 ms at the copy rate), against 10 x 128 x D operations (1.25 ms): memory.  Measured there: 2.99 ms for the

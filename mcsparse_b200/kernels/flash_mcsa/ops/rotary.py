@@ -56,8 +56,9 @@ class RotaryEmbedding:
     * ``"ntk"``: theta times ``factor**(n/(n-1))``, so that the lowest frequency would be divided by ``factor`` and the highest
       stays (one pair: as ``"linear"``);
     * ``"yarn"``: with r the turns that a pair makes over ``original_length`` (one number, or one per axis), frequencies with
-      r >= ``beta_fast`` stay, those with r <= ``beta_slow`` are divided by ``factor``, linear in r between; the rotation is
-      scaled by ``magnitude``, default 0.1 ln(largest factor) + 1 (at least 1).
+      r >= ``beta_fast`` stay, those with r <= ``beta_slow`` are divided by ``factor``, linear in r between (a model that was
+      trained with a ramp in the pair's index instead is rotated differently by this); the rotation is scaled by
+      ``magnitude``, default 0.1 ln(largest factor) + 1 (at least 1).
 
     ``magnitude`` (default 1 except for ``"yarn"``) multiplies the rotated part.
     """
